@@ -1,5 +1,6 @@
 /*
- * reax_abi.h -- the C ABI of the five REAX engine kernel libraries, built for B200 (sm_100a).
+ * reax_abi.h -- the C ABI of the REAX engine kernel libraries, built for B200 (sm_100a): the reference's five, and
+ * libreax_decode.so (EXTENSIONS only).
  *
  * Every entry point below keeps the exact name, argument order and argument meaning of the
  * sm_120 reference library it replaces, so an engine that dlopen()s libreax_*.so and binds these
@@ -165,11 +166,60 @@ int reax_fmha_b_hd(const void* q, const void* k, const void* v, const void* bias
                    long long ksM, long long vsB, long long vsH, long long vsM, long long bsB, long long bsH,
                    long long bsM, long long osB, long long osH, long long osM, int head_dim, void* stream);
 
+/* ---- libreax_decode.so: what a serving step reads and writes ----
+ *
+ * Quantised, paged key/value cache.  A row is the D (128 or 256) values of one token and key/value head.  With n the least
+ * integer >= -127 for which max|x| <= 448 * 2^n it holds e4m3(x / 2^n) (one byte per value) and the exponent byte n + 127;
+ * a row with a value that is not finite holds zeros and the byte 255, and reads back as NaN.
+ * Values kc, vc: row `off` of page p and head h at p*csP + h*csH + off*D; exponents ke, ve: byte p*esP + h*esH + off.
+ * page (rows per page) is a multiple of 16.  Slot of a token: p*page + off.
+ * Codes of all four: -3 head dimension, -2 page size (delta_state: heads), -1 a NULL or unaligned pointer (16 bytes: values,
+ * q, o, state, workspace; attention also exponents), a stride that leaves that alignment, or a size out of range; -4 set-up,
+ * -5 no workspace. */
+
+/* EXTENSION: quantises k and v [T][H][D] bf16 (token and head strides in elements, multiples of 8) into the rows slots[t].
+ * A negative slot is skipped; one past pages*page is skipped and reported by reax_b200_status (0x501).  Slots must differ: where
+ * two tokens of a call name the same one, its row is one of the two, or a mixture. */
+int reax_kv_write(const void* k, long long ksT, long long ksH, const void* v, long long vsT, long long vsH, void* kc,
+                  void* ke, void* vc, void* ve, long long csP, long long csH, long long esP, long long esH,
+                  const long long* slots, int T, int H, int D, int page, long long pages, void* stream);
+/* EXTENSION: reads rows back as bf16 (exact but where the value is past bf16's range).  Rows of negative slots are zeros; so
+ * are those past the end, which are reported. */
+int reax_kv_read(void* k, long long ksT, long long ksH, void* v, long long vsT, long long vsH, const void* kc,
+                 const void* ke, const void* vc, const void* ve, long long csP, long long csH, long long esP,
+                 long long esH, const long long* slots, int T, int H, int D, int page, long long pages, void* stream);
+
+/* EXTENSION: attention over the cache.  Rows as in reax_fmha_q (row r of batch b and key/value head h: token r / G, query head
+ * h*G + r % G).  Position j < prefix_len is row j % page of page prefix[j / page], the same for every sequence and computed once
+ * for all of them; position prefix_len + j is row j % page of page table[b*tsB + j / page], j < P*page.  Row r of batch b sees
+ * the positions <= qpos[b*qpBs + r / G]; a row that sees none is 0.  Keys of a page id outside 0 .. pages-1 are not seen, and
+ * reported (0x502).  ws: 4 * splits * B*H*M * (D + 1) bytes of scratch for the call, splits = reax_fmha_paged_splits(...) of
+ * the same sizes on the current device; it may be NULL where that is 1.  prefix may be NULL where prefix_len is 0. */
+int reax_fmha_paged_splits(int B, int H, int M, int D, int P, int page, int prefix_len);
+int reax_fmha_paged(const void* q, long long qsB, long long qsH, long long qsM, const void* kc, const void* ke,
+                    const void* vc, const void* ve, long long csP, long long csH, long long esP, long long esH,
+                    const int* table, long long tsB, const int* prefix, int prefix_len, const int* qpos, int G,
+                    long long qpBs, void* o, long long osB, long long osH, long long osM, void* ws, float scale, int B,
+                    int H, int M, int D, int P, int page, long long pages, void* stream);
+
+/* EXTENSION: gated delta rule with a carried state, for sequences of any length from one token on.  Per token, with h the
+ * [128 value][128 key] fp32 state of (sequence, value head) and key head hv / (HV / H):
+ *   h <- 2^g h;  u = beta (v - h k);  h <- h + u k^T;  o = scale * h q
+ * q, k [T][H][128], v, o [T][HV][128], beta [T][HV] bf16; g [T][HV] fp32, the token's own log2 decay (not the chunk-local sum that
+ * reax_howu takes); cu [N+1] int64.  state: slot s, head hv at s*ssS + hv*16384 elements, updated in place; sequence n uses slot
+ * slots[n] (n itself where slots is NULL).  fresh (bytes, may be NULL): a sequence with a nonzero byte starts from zeros, whatever
+ * its slot holds.  A sequence without tokens, or with a negative slot, is left alone: its state and its rows of o.  A sequence
+ * whose slot is >= S, or named by an earlier sequence with tokens, does not run: its rows of o are NaN and it is reported (0x503).
+ * Rows of o behind cu[N] are not written.  HV must be a multiple of H. */
+int reax_delta_state(const void* q, const void* k, const void* v, const void* g, const void* beta, const long long* cu,
+                     void* state, long long ssS, const int* slots, const void* fresh, void* o, float scale, long long T,
+                     long long S, int N, int H, int HV, void* stream);
+
 /* EXTENSION: device status word of the calling library.  Every bounded wait inside this library's kernels
  * that runs out records a nonzero code there (and the kernel returns early instead of hanging).
  * Reads and clears the word in one atomic step on `stream` (a code recorded by a kernel on another stream is
  * never lost between a read and a clear), synchronises `stream` and returns the code.  0 = no timeout seen.
- * Exported by all five. */
+ * Exported by all six. */
 int reax_b200_status(void* stream);
 
 #ifdef __cplusplus

@@ -1,4 +1,4 @@
-"""ctypes binding of the five sm_100a libraries -- the same binding the REAX engine makes to the reference
+"""ctypes binding of the six sm_100a libraries -- the same binding the REAX engine makes to the reference
 libraries (``dlopen`` + symbol lookup by name, raw device pointers and ``cudaStream_t`` passed as integers).
 
 Every prototype mirrors ``include/reax_abi.h`` (which cites the reference definition of each entry point).
@@ -24,6 +24,7 @@ _FMHA_Q = [c_vp, c_vp, c_vp, c_vp, c_int, c_ll, c_vp, c_float, c_int, c_int, c_i
 _FMHA_QP = ([c_vp, c_vp, c_vp, c_vp, c_int, c_ll, c_float, c_int, c_int, c_int, c_int] + [c_ll] * 9 +
             [c_vp, c_int, c_vp, c_ll, c_vp, c_ll, c_vp])
 _HOWU = [c_vp] * 8 + [c_float, c_int, c_int, c_int, c_vp]
+_KV = [c_vp, c_ll, c_ll, c_vp, c_ll, c_ll] + [c_vp] * 4 + [c_ll] * 4 + [c_vp] + [c_int] * 4 + [c_ll, c_vp]
 
 # name -> (restype, argtypes); per library
 PROTOTYPES = {
@@ -71,6 +72,15 @@ PROTOTYPES = {
         "reax_fmha_qp": (c_int, _FMHA_QP),
         "reax_fmha_q_hd": (c_int, _FMHA_Q[:-1] + [c_int, c_vp]),
         "reax_fmha_b_hd": (c_int, _FMHA_B[:-1] + [c_int, c_vp]),
+        "reax_b200_status": (c_int, [c_vp]),
+    },
+    "libreax_decode": {
+        "reax_kv_write": (c_int, _KV),
+        "reax_kv_read": (c_int, _KV),
+        "reax_fmha_paged_splits": (c_int, [c_int] * 7),
+        "reax_fmha_paged": (c_int, [c_vp, c_ll, c_ll, c_ll] + [c_vp] * 4 + [c_ll] * 4 + [c_vp, c_ll, c_vp, c_int, c_vp, c_int,
+                                    c_ll, c_vp, c_ll, c_ll, c_ll, c_vp, c_float] + [c_int] * 6 + [c_ll, c_vp]),
+        "reax_delta_state": (c_int, [c_vp] * 7 + [c_ll] + [c_vp] * 3 + [c_float, c_ll, c_ll, c_int, c_int, c_int, c_vp]),
         "reax_b200_status": (c_int, [c_vp]),
     },
 }

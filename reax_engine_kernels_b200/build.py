@@ -1,4 +1,4 @@
-"""In-tree build of the five sm_100a kernel libraries (and the test oracle).
+"""In-tree build of the six sm_100a kernel libraries (and the test oracle).
 
 Each library is one nvcc translation unit compiled with ``-gencode arch=compute_100a,code=sm_100a`` into
 ``reax_engine_kernels_b200/lib/`` so the built ``.so`` files travel with the source tree.  Builds are
@@ -34,6 +34,7 @@ LIBRARIES = {
     "libreax_slices": "slices.cu",
     "libreax_howu": "howu_lib.cu",
     "libreax_fmha_post": "fmha_post_lib.cu",
+    "libreax_decode": "decode_lib.cu",
 }
 
 

@@ -1,6 +1,6 @@
 // Shared device/host helpers for the sm_100a REAX kernel libraries.
 //
-// Every library (libreax_gv, libreax_plain, libreax_slices, libreax_howu, libreax_fmha_post) is ONE
+// Every library (libreax_gv, libreax_plain, libreax_slices, libreax_howu, libreax_fmha_post, libreax_decode) is ONE
 // translation unit that includes this header once, so the status word below is private to each library.
 //
 // Contents:
@@ -54,6 +54,9 @@ enum StatusCode : unsigned int {
   ST_TIMEOUT_ATTN = 0x201,      // attention pipeline wait
   ST_TIMEOUT_KKT = 0x301,       // KKT gave up waiting for its k k^T accumulator
   ST_TIMEOUT_HOWU = 0x401,      // delta rule gave up waiting for a chunk's MMAs
+  ST_BAD_SLOT = 0x501,          // a cache slot past the cache's end (the row is skipped)
+  ST_BAD_PAGE = 0x502,          // a page id outside the cache (its keys are not seen)
+  ST_BAD_STATE = 0x503,         // a state slot past the pool's end, or one that two sequences name
 };
 
 __device__ __forceinline__ void record_status(unsigned int code) { atomicCAS(&g_status_word, 0u, code); }
