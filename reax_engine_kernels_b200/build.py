@@ -75,11 +75,39 @@ def build_library(name: str, force: bool = False, verbose: bool = False) -> str:
     return out
 
 
+def binding_path() -> str:
+    return os.path.join(LIBDIR, "_serving.so")
+
+
+def build_binding(force: bool = False) -> str:
+    """The torch binding of libreax_decode (host C++ only, linked against that library, which lies beside it)."""
+    src, out = os.path.join(CSRC, "serving_binding.cpp"), binding_path()
+    deps = [src, os.path.join(ROOT, "include", "reax_abi.h")]
+    if not force and os.path.exists(out) and os.path.getmtime(out) >= _newest(deps):
+        return out
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension as ext
+
+    cuda = os.path.dirname(os.path.dirname(NVCC))
+    inc = ext.include_paths() + [sysconfig.get_paths()["include"], os.path.join(cuda, "include"), os.path.join(ROOT, "include")]
+    torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    tmp = out + ".tmp"
+    cmd = (["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"] + [f"-I{p}" for p in inc] + [src, "-o", tmp, f"-L{LIBDIR}",
+            "-l:libreax_decode.so", f"-L{torch_lib}", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"])
+    _run(cmd, "_serving")
+    os.replace(tmp, out)
+    return out
+
+
 def build_libraries(force: bool = False, verbose: bool = False, names=None):
     names = list(names or [n for n, tu in LIBRARIES.items() if os.path.exists(os.path.join(CSRC, tu))])
     with cf.ThreadPoolExecutor(max_workers=len(names) or 1) as ex:
         futs = {ex.submit(build_library, n, force, verbose): n for n in names}
-        return [f.result() for f in cf.as_completed(futs)]
+        built = [f.result() for f in cf.as_completed(futs)]
+    return built + [build_binding(force)] if "libreax_decode" in names else built
 
 
 def build_oracle(force: bool = False):

@@ -251,88 +251,40 @@ def kv_cache(pages: int, H: int, page: int, D: int, device="cuda") -> KvCache:
     return KvCache(k, ke, v, ve)
 
 
-def _want(name, t, dtype, shape, device):
-    """`t` is a tensor of that dtype and device; shape entries that are None may have any size."""
-    if t.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the operands on {device}")
-    if t.dim() != len(shape) or any(w is not None and w != n for w, n in zip(shape, t.shape)):
-        raise ValueError(f"{name} must have shape {tuple('*' if w is None else w for w in shape)}, got {tuple(t.shape)}")
+_serving = None
 
 
-def _check_cache(c, H, D, device):
-    k, ke, v, ve = c
-    page = k.shape[2] if k.dim() == 4 else None
-    _want("cache.k", k, torch.float8_e4m3fn, (None, H, None, D), device)
-    _want("cache.v", v, torch.float8_e4m3fn, k.shape, device)
-    _want("cache.ke", ke, torch.uint8, k.shape[:3], device)
-    _want("cache.ve", ve, torch.uint8, k.shape[:3], device)
-    if k.stride() != v.stride() or ke.stride() != ve.stride():
-        raise ValueError("cache.k and cache.v (and cache.ke and cache.ve) must have the same strides")
-    if page <= 0 or page % 16:
-        raise ValueError(f"the page size must be a multiple of 16, got {page}")
-    if k.stride(3) != 1 or k.stride(2) != D or ke.stride(2) != 1:
-        raise ValueError("the rows of a page and head must be contiguous")
-    return page
+def _binding():
+    """The module _serving (csrc/serving_binding.cpp): checks, allocation and the C call in one step, as serving calls are
+    short (a 64-token kv_write takes 22 us with the checks in Python and the call by ctypes)."""
+    global _serving
+    if _serving is None:
+        import importlib.util
 
+        from .build import binding_path
 
-class _on:
-    """The tensors' device as the current one for the length of a call (the libraries launch on the current device)."""
-
-    def __init__(self, device):
-        i, now = device.index, torch.cuda.current_device()
-        self.prev = None if i == now else now
-        if self.prev is not None:
-            torch.cuda.set_device(i)
-
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        if self.prev is not None:
-            torch.cuda.set_device(self.prev)
-
-
-def _kv_args(k, v, c, slots):
-    T, H, D = k.shape
-    return (k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), c.k.data_ptr(), c.ke.data_ptr(),
-            c.v.data_ptr(), c.ve.data_ptr(), c.k.stride(0), c.k.stride(1), c.ke.stride(0), c.ke.stride(1), slots.data_ptr(),
-            T, H, D, c.k.shape[2], c.k.shape[0], _stream(k.device))
-
-
-def _check_kv(k, v, cache, slots):
-    if k.dim() != 3:
-        raise ValueError(f"k must be [T, H, D], got {tuple(k.shape)}")
-    T, H, D = k.shape
-    _want("k", k, torch.bfloat16, (T, H, D), k.device)
-    _want("v", v, torch.bfloat16, (T, H, D), k.device)
-    _want("slots", slots, torch.int64, (T,), k.device)
-    if D not in (128, 256):
-        raise ValueError(f"the head dimension must be 128 or 256, got {D}")
-    _last_dim_contiguous(k=k, v=v, slots=slots)
-    _check_cache(cache, H, D, k.device)
-    _dev(k)
+        abi.load("libreax_decode")
+        path = binding_path()
+        spec = importlib.util.spec_from_file_location("_serving", path)
+        try:
+            mod = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(mod)
+        except (ImportError, OSError) as e:
+            raise abi.ReaxLibraryError(f"cannot load {path} (run `python -m reax_engine_kernels_b200.build`): {e}") from e
+        _serving = mod
+    return _serving
 
 
 def kv_write(k, v, cache: KvCache, slots) -> None:
     """Quantise k, v [T, H, D] bf16 (any token and head strides that are multiples of 8) into the cache's rows slots [T]
     int64.  Negative slots are skipped, slots past the cache's end too (``status`` then reports 0x501); slots must differ."""
-    _check_kv(k, v, cache, slots)
-    with _on(k.device):
-        _check(abi.load("libreax_decode").reax_kv_write(*_kv_args(k, v, cache, slots)), "reax_kv_write")
+    _check((_serving or _binding()).kv_write(k, v, *cache, slots), "reax_kv_write")
 
 
 def kv_read(cache: KvCache, slots, k=None, v=None):
     """The rows slots [T] int64 of the cache as bf16 k, v [T, H, D]; rows of negative slots are zeros."""
-    if cache.k.dim() != 4 or slots.dim() != 1:
-        raise ValueError(f"cache.k must be [pages, H, page, D] and slots [T], got {tuple(cache.k.shape)}, {tuple(slots.shape)}")
-    shape = (slots.shape[0], cache.k.shape[1], cache.k.shape[3])
-    k = torch.empty(shape, dtype=torch.bfloat16, device=slots.device) if k is None else k
-    v = torch.empty(shape, dtype=torch.bfloat16, device=slots.device) if v is None else v
-    _check_kv(k, v, cache, slots)
-    with _on(k.device):
-        _check(abi.load("libreax_decode").reax_kv_read(*_kv_args(k, v, cache, slots)), "reax_kv_read")
+    rc, k, v = (_serving or _binding()).kv_read(*cache, slots, k, v)
+    _check(rc, "reax_kv_read")
     return k, v
 
 
@@ -340,43 +292,9 @@ def fmha_paged(q, cache: KvCache, table, scale: float, *, qpos, G: int = 1, pref
     """Attention of a few tokens per sequence over the quantised cache.  q [B, H, M, D] bf16 as in ``fmha`` (row r = token
     r / G, query head h*G + r % G); table [B, P] int32 page ids of each sequence's own positions; qpos [B, *] int32, row r
     sees positions <= qpos[b, r / G].  With a prefix (int32 page ids, shared by the batch and computed once for all of it) the
-    positions 0 .. prefix_len-1 are its rows and the sequences' own positions start at prefix_len.  A row that sees no key is 0."""
-    if q.dim() != 4:
-        raise ValueError(f"q must be [B, H, M, D], got {tuple(q.shape)}")
-    B, H, M, D = q.shape
-    dev = q.device
-    _want("q", q, torch.bfloat16, (B, H, M, D), dev)
-    if D not in (128, 256):
-        raise ValueError(f"the head dimension must be 128 or 256, got {D}")
-    page = _check_cache(cache, H, D, dev)
-    _want("table", table, torch.int32, (B, None), dev)
-    _want("qpos", qpos, torch.int32, (B, None), dev)
-    if G <= 0 or M % G or qpos.shape[1] < M // G:
-        raise ValueError(f"G = {G} must divide M = {M}, and qpos needs M / G columns, got {qpos.shape[1]}")
-    if prefix is None:
-        if prefix_len:
-            raise ValueError("prefix_len without a prefix")
-    else:
-        _want("prefix", prefix, torch.int32, (None,), dev)
-        if not 0 <= prefix_len <= prefix.shape[0] * page:
-            raise ValueError(f"prefix_len = {prefix_len}, but the prefix has {prefix.shape[0]} pages of {page}")
-        _last_dim_contiguous(prefix=prefix)
-    if out is None:
-        out = torch.empty(B, H, M, D, dtype=torch.bfloat16, device=dev)
-    else:
-        _want("out", out, torch.bfloat16, (B, H, M, D), dev)
-    _last_dim_contiguous(q=q, out=out, table=table, qpos=qpos)
-    _dev(q)
-    lib = abi.load("libreax_decode")
-    k, ke, v, ve = cache
-    P = table.shape[1]
-    with _on(dev):
-        n = lib.reax_fmha_paged_splits(B, H, M, D, P, page, prefix_len)
-        ws = torch.empty(n * B * H * M * (D + 1), dtype=torch.float32, device=dev) if n > 1 else None
-        rc = lib.reax_fmha_paged(q.data_ptr(), *_s3(q), k.data_ptr(), ke.data_ptr(), v.data_ptr(), ve.data_ptr(), k.stride(0),
-                                 k.stride(1), ke.stride(0), ke.stride(1), table.data_ptr(), table.stride(0), _ptr(prefix),
-                                 prefix_len, qpos.data_ptr(), G, qpos.stride(0), out.data_ptr(), *_s3(out), _ptr(ws), scale, B,
-                                 H, M, D, P, page, k.shape[0], _stream(dev))
+    positions 0 .. prefix_len-1 are its rows and the sequences' own positions start at prefix_len.  A row that sees no key is 0;
+    keys of a page id outside the cache are not seen (``status`` then reports 0x502)."""
+    rc, out = (_serving or _binding()).fmha_paged(q, *cache, table, scale, qpos, G, prefix, prefix_len, out)
     _check(rc, "reax_fmha_paged")
     return out
 
@@ -388,39 +306,6 @@ def delta_state(q, k, v, g, beta, cu, scale: float, state, *, slots=None, fresh=
     [S, HV, 128 (value), 128 (key)] fp32, updated in place: sequence n uses slot slots[n] (int32; n without slots).  fresh [N]
     bool: those sequences start from zeros.  Sequences without tokens or with a negative slot are left alone; one whose slot is
     past the end or already taken by an earlier sequence gets NaN rows, and ``status`` reports 0x503.  Returns o [T, HV, 128]."""
-    if q.dim() != 3 or v.dim() != 3 or cu.dim() != 1 or cu.shape[0] < 1:
-        raise ValueError("q, k, v must be [T, heads, 128] and cu [N + 1]")
-    T, H, _ = q.shape
-    HV, N, dev = v.shape[1], cu.shape[0] - 1, q.device
-    if H <= 0 or HV <= 0 or HV % H:
-        raise ValueError(f"the value heads ({HV}) must be a multiple of the key heads ({H})")
-    _want("q", q, torch.bfloat16, (T, H, 128), dev)
-    _want("k", k, torch.bfloat16, (T, H, 128), dev)
-    _want("v", v, torch.bfloat16, (T, HV, 128), dev)
-    _want("beta", beta, torch.bfloat16, (T, HV), dev)
-    _want("g", g, torch.float32, (T, HV), dev)
-    _want("cu", cu, torch.int64, (N + 1,), dev)
-    _want("state", state, torch.float32, (None, HV, 128, 128), dev)
-    if slots is not None:
-        _want("slots", slots, torch.int32, (N,), dev)
-    elif N > state.shape[0]:
-        raise ValueError(f"{N} sequences, but the state has {state.shape[0]} slots")
-    if state.shape[0] > 1 and state.stride(0) < HV * 128 * 128:
-        raise ValueError("the state's slots overlap")
-    if fresh is not None:
-        _want("fresh", fresh, torch.bool, (N,), dev)
-    if o is None:
-        o = torch.empty(T, HV, 128, dtype=torch.bfloat16, device=dev)
-    else:
-        _want("o", o, torch.bfloat16, (T, HV, 128), dev)
-    for name, t in (("q", q), ("k", k), ("v", v), ("beta", beta), ("g", g), ("cu", cu), ("o", o), ("state", state[0] if state.shape[0] else state),
-                    ("slots", slots), ("fresh", fresh)):
-        if t is not None and not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous" + (" within a slot" if name == "state" else ""))
-    _dev(q)
-    with _on(dev):
-        rc = abi.load("libreax_decode").reax_delta_state(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), cu.data_ptr(), state.data_ptr(),
-            state.stride(0), _ptr(slots), _ptr(fresh), o.data_ptr(), scale, T, state.shape[0], N, H, HV, _stream(dev))
+    rc, o = (_serving or _binding()).delta_state(q, k, v, g, beta, cu, scale, state, slots, fresh, o)
     _check(rc, "reax_delta_state")
     return o
