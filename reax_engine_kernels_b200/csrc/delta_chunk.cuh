@@ -1,0 +1,443 @@
+// Gated delta rule with a carried state over 32-token chunks, for sequences longer than a few tokens (see delta_state.cuh for the
+// recurrence, the arguments and the kernel for short ones), sm_100a.
+//
+// With G_i the log2 decay from the chunk's start through token i, and h the state before the chunk, the chunk's updates solve
+//   u_i = beta_i (v_i - 2^G_i h k_i - sum_{j<i} 2^(G_i - G_j) (k_i . k_j) u_j)
+// that is, u = T r with T = (1 + L)^-1 diag(beta), L_ij = beta_i 2^(G_i - G_j) (k_i . k_j) below the diagonal, r_j = v_j - 2^G_j h k_j;
+//   o_i = scale (2^G_i h q_i + sum_{j<=i} 2^(G_i - G_j) (q_i . k_j) u_j),  h <- 2^G_last h + sum_j 2^(G_last - G_j) u_j k_j^T.
+//
+// Precision.  The state is fp32 and stays so: k and q are bf16 and enter the matrix products as they are; an fp32 operand (h, r, u,
+// T) enters as the sum of three bf16 numbers, which hold its 24 bits, one product each (of products of two such operands the six
+// that reach 2^-24).  What only feeds o, which is rounded to bf16, takes two.  The products accumulate in fp32.  G is summed in 64
+// bits: a difference of sums of strong decays would lose its low bits in 32.  An infinity or NaN in a token's inputs may reach the
+// outputs of all tokens of its chunk.
+//
+// Bound: the tensor pipe of mma.sync.  A warp owns 16 rows of h in accumulator fragments (64 registers), which are at once
+// the layout of the A operand of h k, so the state never leaves the registers; 310 m16n8k16 per warp and chunk, 8 cycles
+// each.  (tcgen05 would want 128 rows and the state in tensor memory, to be read, split and written back each chunk; three
+// bf16 terms at 16 rows keep it in place.)  A CTA is 64 rows of one (sequence, head): four such warps, and two that
+// prepare the next chunk (copies, the two Gram matrices, decays, the triangular inverse) while the four work on
+// this one, with one barrier per chunk.  Two CTAs per SM.
+#pragma once
+#include "delta_state.cuh"
+
+namespace reax {
+
+constexpr int DC_T = 32;                 // tokens per chunk
+constexpr int DC_THREADS = 192;
+constexpr int DC_KP = 272, DC_VP = 144;  // row pitches in bytes of k, q and of v: 16 past a multiple of 128, so that eight rows of an
+constexpr int DC_MP = 80;                // ldmatrix fall in different banks; of T and of P (32 bf16)
+struct DcIn {                            // a chunk's inputs
+  uint8_t k[DC_T * DC_KP], q[DC_T * DC_KP], v[DC_T * DC_VP];
+};
+struct DcPrep {  // what is prepared of them
+  uint8_t T[3][DC_T * DC_MP], P[2][DC_T * DC_MP];
+  float grow[DC_T], left[DC_T];  // 2^G_i, 2^(G_last - G_i)
+};
+struct DcSmem {
+  DcIn in[3];
+  DcPrep prep[2];
+  double G[2][DC_T];
+  float L[DC_T][DC_T + 1];
+  float beta[DC_T];
+  uint8_t o[4][DC_T * 48];  // per warp: 32 tokens x 16 rows
+};
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void stsm_x4_t(uint32_t addr, const uint32_t (&r)[4]) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3])
+               : "memory");
+}
+// x, y as sums of N bf16 numbers: s[i] holds the i-th terms of both (8, 16 or 24 bits in all)
+template <int N>
+__device__ __forceinline__ void split_bf16(float x, float y, uint32_t (&s)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    s[i] = pack_bf16(x, y);
+    if (i + 1 < N) {
+      x -= bf_lo(s[i]);
+      y -= bf_hi(s[i]);
+    }
+  }
+}
+// accumulator fragments of two n8 tiles -> the A fragment of one k16 step, in N terms
+template <int N>
+__device__ __forceinline__ void split_frag(const float (&c0)[4], const float (&c1)[4], uint32_t (&a)[N][4]) {
+  uint32_t s[N];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const float(&c)[4] = r < 2 ? c0 : c1;
+    split_bf16<N>(c[(r & 1) * 2], c[(r & 1) * 2 + 1], s);
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[i][r] = s[i];
+  }
+}
+
+// copies of the 32 tokens from t on into `in`, zeros past the sequence's end; threads 0..63
+__device__ __forceinline__ void dc_load(const DeltaArgs& a, DcIn& in, long long t, long long e, int hk, int hv, int row0, int tid) {
+  const long long kT = (long long)a.H * 128, vT = (long long)a.HV * 128;
+  const int c = tid & 15;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = (tid >> 4) + 4 * i;
+    const bool ok = t + r < e;
+    const long long off = (ok ? t + r : t) * kT + hk * 128 + c * 8;
+    cp_async16(smem_u32(in.k + r * DC_KP + c * 16), a.k + off, ok);
+    cp_async16(smem_u32(in.q + r * DC_KP + c * 16), a.q + off, ok);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = (tid >> 3) + 8 * i;
+    const bool ok = t + r < e;
+    cp_async16(smem_u32(in.v + r * DC_VP + (tid & 7) * 16), a.v + (ok ? t + r : t) * vT + hv * 128 + row0 + (tid & 7) * 8, ok);
+  }
+}
+
+// One of the two preparing warps: w = 0 the inverse T (from k . k), w = 1 the products P (from q . k) and the decays.
+__device__ __forceinline__ void dc_prepare(DcSmem& s, const DcIn& in, DcPrep& out, int w, int lane, float g, float beta) {
+  const int gq = lane >> 2, t = lane & 3;
+  // G_i: a token's decay below 2^-1000 is nothing in fp32, and keeps the sums finite
+  double G = g < -1000.f ? -1000.0 : (double)g;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double x = __shfl_up_sync(0xffffffffu, G, o);
+    if (lane >= o) G += x;
+  }
+  s.G[w][lane] = G;
+  if (w == 1) {
+    out.grow[lane] = exp2f((float)G);
+    out.left[lane] = exp2f((float)(__shfl_sync(0xffffffffu, G, 31) - G));
+  } else {
+    s.beta[lane] = beta;
+  }
+  __syncwarp();
+  // rows i of k (or q) times rows j of k, tiles that touch the lower triangle
+  const uint32_t ka = smem_u32(in.k), xa = w ? smem_u32(in.q) : ka;
+  float acc[2][4][4];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.f;
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks) {
+    uint32_t x[2][4], b[2][4];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      ldsm_x4(xa + (m * 16 + (lane & 15)) * DC_KP + ks * 32 + (lane >> 4) * 16, x[m]);
+      ldsm_x4(ka + (m * 16 + (lane & 7) + (lane >> 4) * 8) * DC_KP + ks * 32 + ((lane >> 3) & 1) * 16, b[m]);
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int n = 0; n < 2 * (m + 1); ++n) mma_bf16(acc[m][n], x[m], b[n >> 1][(n & 1) * 2], b[n >> 1][(n & 1) * 2 + 1]);
+  }
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int i = m * 16 + gq + 8 * r, j = n * 8 + 2 * t;
+        const double Gi = s.G[w][i];
+        float x[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const bool in_tri = w ? j + e <= i : j + e < i;
+          x[e] = in_tri ? acc[m][n][2 * r + e] * exp2f((float)(Gi - s.G[w][j + e])) : 0.f;
+        }
+        if (w) {
+          uint32_t p[2];
+          split_bf16<2>(x[0], x[1], p);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) *reinterpret_cast<uint32_t*>(out.P[k] + i * DC_MP + j * 2) = p[k];
+        } else {
+          const float bi = s.beta[i];
+          s.L[i][j] = bi * x[0];
+          s.L[i][j + 1] = bi * x[1];
+        }
+      }
+    }
+  if (w) return;
+  __syncwarp();
+  // column `lane` of (1 + L)^-1 by forward substitution, right-looking: once x_j is final, it leaves the later ones
+  float x[DC_T];
+#pragma unroll
+  for (int i = 0; i < DC_T; ++i) x[i] = i == lane ? 1.f : 0.f;
+#pragma unroll
+  for (int j = 0; j < DC_T - 1; ++j)
+#pragma unroll
+    for (int i = j + 1; i < DC_T; ++i) x[i] = __fmaf_rn(-s.L[i][j], x[j], x[i]);
+#pragma unroll
+  for (int i = 0; i < DC_T; ++i) {
+    float y = x[i] * beta;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      const uint16_t b = __bfloat16_as_ushort(__float2bfloat16_rn(y));
+      *reinterpret_cast<uint16_t*>(out.T[k] + i * DC_MP + lane * 2) = b;
+      y -= bf_lo(b);
+    }
+  }
+}
+
+// grid (2, HV, N): 64 rows of one (sequence, value head) per CTA; sequences of at most DS_MOST tokens are the step kernel's
+__global__ void __launch_bounds__(DC_THREADS, 2) delta_chunk_kernel(DeltaArgs a) {
+  extern __shared__ __align__(128) uint8_t dc_raw[];
+  DcSmem& s = *reinterpret_cast<DcSmem*>(dc_raw);
+  const int n = blockIdx.z, hv = blockIdx.y, lane = threadIdx.x & 31, warp = warp_id();
+  const int gq = lane >> 2, t4 = lane & 3, row0 = blockIdx.x * 64;
+  long long t0, e;
+  delta_range(a, n, t0, e);
+  if (e - t0 <= DS_MOST) return;
+  const int slot = delta_slot(a, n);
+  if (slot == -1) return;
+  const long long oT = (long long)a.HV * 128;
+  if (slot < 0) {  // the rows of a sequence that cannot run are NaN
+    uint16_t* o = a.o + (long long)hv * 128 + row0;
+    for (long long i = threadIdx.x; i < (e - t0) * 64; i += DC_THREADS) o[(t0 + (i >> 6)) * oT + (i & 63)] = 0x7fff;
+    return;
+  }
+  const int hk = hv / (a.HV / a.H);
+  const int chunks = (int)((e - t0 + DC_T - 1) / DC_T);
+  const int pt = threadIdx.x - 128;  // preparing threads: 0..63
+  float gw = 0.f, bw = 0.f;          // their token's decay and beta, a chunk ahead
+  auto scalars = [&](int c) {
+    const long long t = t0 + (long long)c * DC_T + lane;
+    gw = t < e ? a.g[t * a.HV + hv] : 0.f;
+    bw = t < e ? bf_lo(a.beta[t * a.HV + hv]) : 0.f;
+  };
+
+  float h[16][4];
+  if (warp >= 4) {
+    dc_load(a, s.in[0], t0, e, hk, hv, row0, pt);
+    cp_async_commit();
+    if (chunks > 1) dc_load(a, s.in[1], t0 + DC_T, e, hk, hv, row0, pt);
+    cp_async_commit();
+    scalars(0);
+    cp_async_wait<1>();
+    named_bar_sync<1, 64>();
+    dc_prepare(s, s.in[0], s.prep[0], warp - 4, lane, gw, bw);
+    scalars(1);
+  } else {
+    const float* st = a.state + slot * a.sS + ((long long)hv * 128 + row0 + warp * 16 + gq) * 128 + 2 * t4;
+    const bool fresh = a.fresh && a.fresh[n];
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float2 x = fresh ? make_float2(0.f, 0.f) : *reinterpret_cast<const float2*>(st + r * 8 * 128 + j * 8);
+        h[j][2 * r] = x.x;
+        h[j][2 * r + 1] = x.y;
+      }
+  }
+  __syncthreads();
+
+  for (int c = 0; c < chunks; ++c) {
+    if (warp >= 4) {
+      if (c + 2 < chunks) dc_load(a, s.in[(c + 2) % 3], t0 + (long long)(c + 2) * DC_T, e, hk, hv, row0, pt);
+      cp_async_commit();
+      if (c + 1 < chunks) {
+        cp_async_wait<1>();
+        named_bar_sync<1, 64>();  // both warps' copies of the chunk have landed
+        const float g = gw, b = bw;
+        scalars(c + 2);
+        dc_prepare(s, s.in[(c + 1) % 3], s.prep[(c + 1) & 1], warp - 4, lane, g, b);
+      }
+    } else {
+      const DcIn& in = s.in[c % 3];
+      const DcPrep& pr = s.prep[c & 1];
+      const uint32_t ka = smem_u32(in.k), qa = smem_u32(in.q), va = smem_u32(in.v);
+      // ---- h k (three terms) and h q (two)
+      float sk[4][4], sq[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) sk[j][x] = sq[j][x] = 0.f;
+      const uint32_t brow = ((lane & 7) + (lane >> 4) * 8) * DC_KP + ((lane >> 3) & 1) * 16;
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) {
+        uint32_t ha[3][4];
+        split_frag<3>(h[2 * ks], h[2 * ks + 1], ha);
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          uint32_t b[4];
+          ldsm_x4(ka + brow + p * 16 * DC_KP + ks * 32, b);
+#pragma unroll
+          for (int i = 2; i >= 0; --i) {
+            mma_bf16(sk[2 * p], ha[i], b[0], b[1]);
+            mma_bf16(sk[2 * p + 1], ha[i], b[2], b[3]);
+          }
+          ldsm_x4(qa + brow + p * 16 * DC_KP + ks * 32, b);
+#pragma unroll
+          for (int i = 1; i >= 0; --i) {
+            mma_bf16(sq[2 * p], ha[i], b[0], b[1]);
+            mma_bf16(sq[2 * p + 1], ha[i], b[2], b[3]);
+          }
+        }
+      }
+      // ---- r = v - 2^G (h k); o starts as 2^G (h q)
+      const uint32_t vaddr = va + ((lane & 7) + (lane >> 4) * 8) * DC_VP + warp * 32 + ((lane >> 3) & 1) * 16;
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        uint32_t vv[4];  // (tokens 0-7, rows 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15)
+        ldsm_x4_t(vaddr + p * 16 * DC_VP, vv);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float2 gr = *reinterpret_cast<const float2*>(&pr.grow[(2 * p + x) * 8 + 2 * t4]);
+          float(&k4)[4] = sk[2 * p + x];
+          float(&q4)[4] = sq[2 * p + x];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            k4[2 * r] = __fmaf_rn(-gr.x, k4[2 * r], bf_lo(vv[2 * x + r]));
+            k4[2 * r + 1] = __fmaf_rn(-gr.y, k4[2 * r + 1], bf_hi(vv[2 * x + r]));
+            q4[2 * r] *= gr.x;
+            q4[2 * r + 1] *= gr.y;
+          }
+        }
+      }
+      // ---- u = T r: the six products of three terms by three
+      float u[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) u[j][x] = 0.f;
+      const uint32_t mrow = ((lane & 7) + (lane >> 4) * 8) * DC_MP + ((lane >> 3) & 1) * 16;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        uint32_t ra[3][4];
+        split_frag<3>(sk[2 * ks], sk[2 * ks + 1], ra);
+#pragma unroll
+        for (int p = ks; p < 2; ++p)
+#pragma unroll
+          for (int y = 2; y >= 0; --y) {
+            uint32_t b[4];
+            ldsm_x4(smem_u32(pr.T[y]) + mrow + p * 16 * DC_MP + ks * 32, b);
+#pragma unroll
+            for (int i = 2 - y; i >= 0; --i) {
+              mma_bf16(u[2 * p], ra[i], b[0], b[1]);
+              mma_bf16(u[2 * p + 1], ra[i], b[2], b[3]);
+            }
+          }
+      }
+      // ---- o += P u
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        uint32_t ua[2][4];
+        split_frag<2>(u[2 * ks], u[2 * ks + 1], ua);
+#pragma unroll
+        for (int p = ks; p < 2; ++p)
+#pragma unroll
+          for (int y = 1; y >= 0; --y) {
+            uint32_t b[4];
+            ldsm_x4(smem_u32(pr.P[y]) + mrow + p * 16 * DC_MP + ks * 32, b);
+#pragma unroll
+            for (int i = 1 - y; i >= 0; --i) {
+              mma_bf16(sq[2 * p], ua[i], b[0], b[1]);
+              mma_bf16(sq[2 * p + 1], ua[i], b[2], b[3]);
+            }
+          }
+      }
+      const uint32_t so = smem_u32(s.o[warp]);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        uint32_t y[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          y[x] = pack_bf16(sq[2 * p + (x >> 1)][(x & 1) * 2] * a.scale, sq[2 * p + (x >> 1)][(x & 1) * 2 + 1] * a.scale);
+        stsm_x4_t(so + (p * 16 + (lane & 7) + (lane >> 4) * 8) * 48 + ((lane >> 3) & 1) * 16, y);
+      }
+      __syncwarp();
+      const long long t = t0 + (long long)c * DC_T + lane;
+      if (t < e) {
+        uint4* dst = reinterpret_cast<uint4*>(a.o + t * oT + hv * 128 + row0 + warp * 16);
+        dst[0] = *reinterpret_cast<const uint4*>(s.o[warp] + lane * 48);
+        dst[1] = *reinterpret_cast<const uint4*>(s.o[warp] + lane * 48 + 16);
+      }
+      // ---- h <- 2^G_last h + (2^(G_last - G_j) u_j) k_j^T
+      const float last = pr.grow[DC_T - 1];
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) h[j][x] *= last;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float2 le = *reinterpret_cast<const float2*>(&pr.left[(2 * ks + x) * 8 + 2 * t4]);
+          float(&u4)[4] = u[2 * ks + x];
+          u4[0] *= le.x, u4[1] *= le.y, u4[2] *= le.x, u4[3] *= le.y;
+        }
+        uint32_t ua[3][4];
+        split_frag<3>(u[2 * ks], u[2 * ks + 1], ua);
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+          uint32_t b[4];  // (tokens 0-7, keys 0-7), (8-15, 0-7), (0-7, 8-15), (8-15, 8-15)
+          ldsm_x4_t(ka + (ks * 16 + (lane & 15)) * DC_KP + j * 16 + (lane >> 4) * 16, b);
+#pragma unroll
+          for (int i = 2; i >= 0; --i) {
+            mma_bf16(h[j], ua[i], b[0], b[1]);
+            mma_bf16(h[j + 1], ua[i], b[2], b[3]);
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if (warp < 4) {
+    float* st = a.state + slot * a.sS + ((long long)hv * 128 + row0 + warp * 16 + gq) * 128 + 2 * t4;
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+        *reinterpret_cast<float2*>(st + r * 8 * 128 + j * 8) = make_float2(h[j][2 * r], h[j][2 * r + 1]);
+  }
+}
+
+}  // namespace reax
+
+namespace reax_host {
+
+inline int delta_go(const reax::DeltaArgs& a, cudaStream_t st) {
+  if (int rc = delta_check(a)) return rc;
+  if (a.N == 0 || a.T == 0) return 0;
+  const dim3 grid(2, a.HV, a.N);
+  // Each kernel takes the sequences of its lengths, which are on the device.  T = N is taken for a decode batch and T <= DS_MOST
+  // leaves no long sequence: the step kernel alone then takes every length.
+  if (a.T == a.N || a.T <= reax::DS_MOST) {
+    reax::delta_step_kernel<<<grid, reax::DS_THREADS, 0, st>>>(a, 0x7fffffffffffffffLL);
+    return (int)cudaGetLastError();
+  }
+  static SmemAttr attr;
+  if (ensure_smem(attr, reax::delta_chunk_kernel, (int)sizeof(reax::DcSmem), true) != cudaSuccess) return -4;
+  reax::delta_chunk_kernel<<<grid, reax::DC_THREADS, sizeof(reax::DcSmem), st>>>(a);
+  reax::delta_step_kernel<<<grid, reax::DS_THREADS, 0, st>>>(a, reax::DS_MOST);
+  return (int)cudaGetLastError();
+}
+
+}  // namespace reax_host
+
+#define REAX_DEFINE_DELTA_STATE_EXPORT()                                                                               \
+  REAX_API int reax_delta_state(const void* q, const void* k, const void* v, const void* g, const void* beta,             \
+                                const long long* cu, void* state, long long ssS, const int* slots, const void* fresh,     \
+                                void* o, float scale, long long T, long long S, int N, int H, int HV, void* stream) {     \
+    reax::DeltaArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (const uint16_t*)beta, (const float*)g,  \
+                      cu, (float*)state, ssS, slots, (const uint8_t*)fresh, (uint16_t*)o, scale, T, S, N, H, HV};          \
+    return reax_host::delta_go(a, (cudaStream_t)stream);                                                                  \
+  }

@@ -32,6 +32,7 @@ struct DeltaArgs {
 };
 
 constexpr int DS_THREADS = 128;
+constexpr long long DS_MOST = 8;  // longest sequence that goes token by token beside longer ones
 
 // The sequence's token range, cut to the T rows there are.
 __device__ __forceinline__ void delta_range(const DeltaArgs& a, int n, long long& b, long long& e) {
@@ -59,14 +60,14 @@ __device__ __forceinline__ int delta_slot(const DeltaArgs& a, int n) {
   return s;
 }
 
-// grid (2, HV, N): 64 rows of one (sequence, value head) per CTA
-__global__ void __launch_bounds__(DS_THREADS) delta_step_kernel(DeltaArgs a) {
+// grid (2, HV, N): 64 rows of one (sequence, value head) per CTA; sequences of more than `most` tokens are the chunk kernel's
+__global__ void __launch_bounds__(DS_THREADS) delta_step_kernel(DeltaArgs a, long long most) {
   const int n = blockIdx.z, hv = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int sub = lane & 15, half = lane >> 4, own = sub >> 1;
   const int row0 = blockIdx.x * 64 + warp * 16 + half * 8;
   long long t, e;
   delta_range(a, n, t, e);
-  if (t >= e) return;
+  if (t >= e || e - t > most) return;
   const int slot = delta_slot(a, n);
   if (slot == -1) return;
   uint16_t* o = a.o + (long long)hv * 128 + row0 + own;
@@ -165,26 +166,10 @@ inline int delta_check(const reax::DeltaArgs& a) {
   if (a.N < 0 || a.N > 65535 || a.T < 0 || a.S < 0) return -1;
   if (a.N == 0 || a.T == 0) return 0;
   if (!a.q || !a.k || !a.v || !a.beta || !a.g || !a.cu || !a.state || !a.o) return -1;
-  if (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.state) & 15) return -1;
+  if (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.o | (uintptr_t)a.state) & 15) return -1;
   if (a.sS % 4) return -1;
   if (!a.slots && a.N > a.S) return -1;
   return 0;
 }
 
-inline int delta_go(const reax::DeltaArgs& a, cudaStream_t st) {
-  if (int rc = delta_check(a)) return rc;
-  if (a.N == 0 || a.T == 0) return 0;
-  reax::delta_step_kernel<<<dim3(2, a.HV, a.N), reax::DS_THREADS, 0, st>>>(a);
-  return (int)cudaGetLastError();
-}
-
 }  // namespace reax_host
-
-#define REAX_DEFINE_DELTA_STATE_EXPORT()                                                                               \
-  REAX_API int reax_delta_state(const void* q, const void* k, const void* v, const void* g, const void* beta,             \
-                                const long long* cu, void* state, long long ssS, const int* slots, const void* fresh,     \
-                                void* o, float scale, long long T, long long S, int N, int H, int HV, void* stream) {     \
-    reax::DeltaArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (const uint16_t*)beta, (const float*)g,  \
-                      cu, (float*)state, ssS, slots, (const uint8_t*)fresh, (uint16_t*)o, scale, T, S, N, H, HV};          \
-    return reax_host::delta_go(a, (cudaStream_t)stream);                                                                  \
-  }

@@ -448,7 +448,7 @@ def assert_delta(d, scale, o, state0, live, slots=None, fresh=None):
 
 @pytest.mark.parametrize("H,HV,lens", [
     (1, 1, [1]), (2, 4, [1, 1, 1]), (4, 4, [2, 0, 3]), (1, 4, [5, 17, 1, 16]), (2, 6, [64, 1, 33]), (16, 32, [1] * 9),
-    (2, 4, [200, 129]), (1, 2, [1000]),
+    (2, 4, [200, 129]), (1, 2, [1000]), (2, 2, [8, 9, 31, 0, 32, 1, 33]), (1, 3, [65, 2, 96, 95]),
 ])
 @pytest.mark.parametrize("fresh", [False, True])
 def test_delta_state(H, HV, lens, fresh):
@@ -547,6 +547,33 @@ def test_delta_state_as_the_chunked_kernels():
     got = rk.delta_state(q, k, v, per, beta, cu, 0.0884, state, fresh=torch.ones(2, dtype=torch.bool, device=DEV))
     assert (got.double() - want.double()).norm() <= 8 * 2.0 ** -8 * want.double().norm()
     assert torch.isfinite(state).all()
+
+
+def test_delta_state_short_sequence_and_rows_behind_it():
+    """One sequence that is much shorter than the rows there are; T = N with uneven lengths."""
+    for lens, behind in (([3], 60), ([50, 0, 0, 1] + [0] * 47, 0)):
+        d = delta_inputs(31, lens, 1, 2, len(lens), behind=behind)
+        state0 = d["state"].clone()
+        o = torch.full((sum(lens) + behind, 2, 128), 7.0, dtype=BF, device=DEV)
+        rk.delta_state(*(d[n] for n in ("q", "k", "v", "g", "beta", "cu")), 0.3, d["state"], o=o)
+        assert (o[sum(lens):] == 7).all()
+        assert_delta(d, 0.3, o, state0, slice(0, sum(lens)))
+
+
+def test_delta_state_sequences_do_not_reach_each_other():
+    """NaN inputs of one sequence, and of the rows behind the last one, stay there."""
+    lens = [40, 5, 70, 3]
+    d = delta_inputs(32, lens, 2, 4, 4, behind=4)
+    clean = {n: t.clone() for n, t in d.items()}
+    for n in ("q", "k", "v", "g", "beta"):
+        d[n][40:45] = math.nan
+        d[n][118:] = math.nan
+    state0 = d["state"].clone()
+    o = rk.delta_state(*(d[n] for n in ("q", "k", "v", "g", "beta", "cu")), 1.0, d["state"])
+    assert torch.isnan(d["state"][1]).all()
+    d["state"][1] = delta_ref({**clean, "state": state0}, 1.0)[2][1].float()
+    live = torch.tensor([t for t in range(118) if not 40 <= t < 45], device=DEV)
+    assert_delta({**clean, "state": d["state"]}, 1.0, o, state0, live)
 
 
 def test_delta_state_graph_and_streams():
