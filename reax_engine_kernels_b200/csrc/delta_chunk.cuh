@@ -8,9 +8,9 @@
 //
 // Precision.  The state is fp32 and stays so: k and q are bf16 and enter the matrix products as they are; an fp32 operand (h, r, u,
 // T) enters as the sum of three bf16 numbers, which hold its 24 bits, one product each (of products of two such operands the six
-// that reach 2^-24).  What only feeds o, which is rounded to bf16, takes two.  The products accumulate in fp32.  G is summed in 64
-// bits: a difference of sums of strong decays would lose its low bits in 32.  An infinity or NaN in a token's inputs may reach the
-// outputs of all tokens of its chunk.
+// that reach 2^-24).  What only feeds o, which is rounded to bf16, takes two.  The products accumulate in fp32.  G is summed in 64-bit
+// fixed point (32 bits behind the point): in fp32 a difference of sums of strong decays would lose its low bits, and fp64 arithmetic
+// took a third of the preparation's time.  An infinity or NaN in a token's inputs may reach the outputs of all tokens of its chunk.
 //
 // Bound: the tensor pipe of mma.sync.  A warp owns 16 rows of h in accumulator fragments (64 registers), which are at once
 // the layout of the A operand of h k, so the state never leaves the registers; 310 m16n8k16 per warp and chunk, 8 cycles
@@ -37,8 +37,8 @@ struct DcPrep {  // what is prepared of them
 struct DcSmem {
   DcIn in[3];
   DcPrep prep[2];
-  double G[2][DC_T];
-  float L[DC_T][DC_T + 1];
+  long long G[2][DC_T];
+  float L[DC_T][DC_T + 4];  // column by column
   float beta[DC_T];
   uint8_t o[4][DC_T * 48];  // per warp: 32 tokens x 16 rows
 };
@@ -89,40 +89,49 @@ __device__ __forceinline__ void split_frag(const float (&c0)[4], const float (&c
   }
 }
 
-// copies of the 32 tokens from t on into `in`, zeros past the sequence's end; threads 0..63
-__device__ __forceinline__ void dc_load(const DeltaArgs& a, DcIn& in, long long t, long long e, int hk, int hv, int row0, int tid) {
-  const long long kT = (long long)a.H * 128, vT = (long long)a.HV * 128;
-  const int c = tid & 15;
+// copies of the 32 tokens from t on into `in`, zeros past the sequence's end; all threads
+__device__ __forceinline__ void dc_load(const DeltaArgs& a, DcIn& in, long long t, long long e, int hk, int hv, int row0) {
+  const int kT = a.H * 128, vT = a.HV * 128, left = (int)min(e - t, (long long)DC_T);
+  const uint16_t *k = a.k + t * kT + hk * 128, *q = a.q + t * kT + hk * 128, *v = a.v + t * vT + hv * 128 + row0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = (tid >> 4) + 4 * i;
-    const bool ok = t + r < e;
-    const long long off = (ok ? t + r : t) * kT + hk * 128 + c * 8;
-    cp_async16(smem_u32(in.k + r * DC_KP + c * 16), a.k + off, ok);
-    cp_async16(smem_u32(in.q + r * DC_KP + c * 16), a.q + off, ok);
+  for (int i = 0; i < (DC_T * 16 + DC_THREADS - 1) / DC_THREADS; ++i) {
+    const int x = threadIdx.x + i * DC_THREADS, r = x >> 4, c = x & 15;
+    if (x < DC_T * 16) {
+      const int off = (r < left ? r : 0) * kT + c * 8;
+      cp_async16(smem_u32(in.k + r * DC_KP + c * 16), k + off, r < left);
+      cp_async16(smem_u32(in.q + r * DC_KP + c * 16), q + off, r < left);
+    }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = (tid >> 3) + 8 * i;
-    const bool ok = t + r < e;
-    cp_async16(smem_u32(in.v + r * DC_VP + (tid & 7) * 16), a.v + (ok ? t + r : t) * vT + hv * 128 + row0 + (tid & 7) * 8, ok);
+  for (int i = 0; i < (DC_T * 8 + DC_THREADS - 1) / DC_THREADS; ++i) {
+    const int x = threadIdx.x + i * DC_THREADS, r = x >> 3, c = x & 7;
+    if (x < DC_T * 8) cp_async16(smem_u32(in.v + r * DC_VP + c * 16), v + (r < left ? r : 0) * vT + c * 8, r < left);
   }
+}
+
+// 2^(x / 2^32): the fraction by ex2, the whole part into the exponent (0 below fp32's normal range, infinity above its range)
+__device__ __forceinline__ float exp2_fixed(long long x) {
+  const int whole = (int)(x >> 32);
+  const float f = ex2_approx((float)((uint32_t)x >> 8) * 0x1p-24f);  // in [1, 2): 24 bits of the fraction are exact in fp32
+  return whole < -126 ? 0.f : whole > 127 ? INFINITY : __uint_as_float(__float_as_uint(f) + ((uint32_t)whole << 23));
 }
 
 // One of the two preparing warps: w = 0 the inverse T (from k . k), w = 1 the products P (from q . k) and the decays.
 __device__ __forceinline__ void dc_prepare(DcSmem& s, const DcIn& in, DcPrep& out, int w, int lane, float g, float beta) {
   const int gq = lane >> 2, t = lane & 3;
-  // G_i: a token's decay below 2^-1000 is nothing in fp32, and keeps the sums finite
-  double G = g < -1000.f ? -1000.0 : (double)g;
+  // G_i.  Past +-2^9 a token's decay is 0 or infinite in fp32 anyway; a NaN one makes its beta NaN
+  const float gc = fminf(fmaxf(g, -512.f), 512.f);
+  long long G = __float2ll_rn(gc * 0x1p32f);
+  if (g != g) beta = g;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const double x = __shfl_up_sync(0xffffffffu, G, o);
+    const long long x = __shfl_up_sync(0xffffffffu, G, o);
     if (lane >= o) G += x;
   }
   s.G[w][lane] = G;
   if (w == 1) {
-    out.grow[lane] = exp2f((float)G);
-    out.left[lane] = exp2f((float)(__shfl_sync(0xffffffffu, G, 31) - G));
+    out.grow[lane] = exp2_fixed(G);
+    out.left[lane] = exp2_fixed(__shfl_sync(0xffffffffu, G, 31) - G);
   } else {
     s.beta[lane] = beta;
   }
@@ -149,19 +158,27 @@ __device__ __forceinline__ void dc_prepare(DcSmem& s, const DcIn& in, DcPrep& ou
 #pragma unroll
       for (int n = 0; n < 2 * (m + 1); ++n) mma_bf16(acc[m][n], x[m], b[n >> 1][(n & 1) * 2], b[n >> 1][(n & 1) * 2 + 1]);
   }
+  long long Gi[2][2], Gj[4][2];  // all read before the first store below, which the compiler would not move them across
+  float bi[2][2];
+#pragma unroll
+  for (int m = 0; m < 4; ++m) {
+    const longlong2 x = *reinterpret_cast<const longlong2*>(&s.G[w][m * 8 + 2 * t]);
+    Gj[m][0] = x.x, Gj[m][1] = x.y;
+    Gi[m >> 1][m & 1] = s.G[w][m * 8 + gq];
+    bi[m >> 1][m & 1] = s.beta[m * 8 + gq];
+  }
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
+    for (int n = 0; n < 2 * (m + 1); ++n)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const int i = m * 16 + gq + 8 * r, j = n * 8 + 2 * t;
-        const double Gi = s.G[w][i];
         float x[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const bool in_tri = w ? j + e <= i : j + e < i;
-          x[e] = in_tri ? acc[m][n][2 * r + e] * exp2f((float)(Gi - s.G[w][j + e])) : 0.f;
+          const float d = acc[m][n][2 * r + e] * exp2_fixed(Gi[m][r] - Gj[n][e]);
+          x[e] = (w ? j + e <= i : j + e < i) ? d : 0.f;
         }
         if (w) {
           uint32_t p[2];
@@ -169,12 +186,10 @@ __device__ __forceinline__ void dc_prepare(DcSmem& s, const DcIn& in, DcPrep& ou
 #pragma unroll
           for (int k = 0; k < 2; ++k) *reinterpret_cast<uint32_t*>(out.P[k] + i * DC_MP + j * 2) = p[k];
         } else {
-          const float bi = s.beta[i];
-          s.L[i][j] = bi * x[0];
-          s.L[i][j + 1] = bi * x[1];
+          s.L[j][i] = -bi[m][r] * x[0];
+          s.L[j + 1][i] = -bi[m][r] * x[1];
         }
       }
-    }
   if (w) return;
   __syncwarp();
   // column `lane` of (1 + L)^-1 by forward substitution, right-looking: once x_j is final, it leaves the later ones
@@ -184,7 +199,13 @@ __device__ __forceinline__ void dc_prepare(DcSmem& s, const DcIn& in, DcPrep& ou
 #pragma unroll
   for (int j = 0; j < DC_T - 1; ++j)
 #pragma unroll
-    for (int i = j + 1; i < DC_T; ++i) x[i] = __fmaf_rn(-s.L[i][j], x[j], x[i]);
+    for (int i = (j + 1) & ~3; i < DC_T; i += 4) {
+      const float4 l = *reinterpret_cast<const float4*>(&s.L[j][i]);  // L is strictly lower: what lies above is not used
+      if (i > j) x[i] = __fmaf_rn(l.x, x[j], x[i]);
+      if (i + 1 > j) x[i + 1] = __fmaf_rn(l.y, x[j], x[i + 1]);
+      if (i + 2 > j) x[i + 2] = __fmaf_rn(l.z, x[j], x[i + 2]);
+      x[i + 3] = __fmaf_rn(l.w, x[j], x[i + 3]);
+    }
 #pragma unroll
   for (int i = 0; i < DC_T; ++i) {
     float y = x[i] * beta;
@@ -216,25 +237,26 @@ __global__ void __launch_bounds__(DC_THREADS, 2) delta_chunk_kernel(DeltaArgs a)
   }
   const int hk = hv / (a.HV / a.H);
   const int chunks = (int)((e - t0 + DC_T - 1) / DC_T);
-  const int pt = threadIdx.x - 128;  // preparing threads: 0..63
-  float gw = 0.f, bw = 0.f;          // their token's decay and beta, a chunk ahead
+  float gw = 0.f;  // the preparing lanes' token's decay and beta (still as bits: a conversion would wait for it), a chunk ahead
+  uint16_t bw = 0;
   auto scalars = [&](int c) {
     const long long t = t0 + (long long)c * DC_T + lane;
     gw = t < e ? a.g[t * a.HV + hv] : 0.f;
-    bw = t < e ? bf_lo(a.beta[t * a.HV + hv]) : 0.f;
+    bw = t < e ? a.beta[t * a.HV + hv] : (uint16_t)0;
   };
 
   float h[16][4];
+  dc_load(a, s.in[0], t0, e, hk, hv, row0);
+  cp_async_commit();
+  if (chunks > 1) dc_load(a, s.in[1], t0 + DC_T, e, hk, hv, row0);
+  cp_async_commit();
+  if (warp >= 4) scalars(0);
+  cp_async_wait<1>();
+  __syncthreads();
   if (warp >= 4) {
-    dc_load(a, s.in[0], t0, e, hk, hv, row0, pt);
-    cp_async_commit();
-    if (chunks > 1) dc_load(a, s.in[1], t0 + DC_T, e, hk, hv, row0, pt);
-    cp_async_commit();
-    scalars(0);
-    cp_async_wait<1>();
-    named_bar_sync<1, 64>();
-    dc_prepare(s, s.in[0], s.prep[0], warp - 4, lane, gw, bw);
+    const float g = gw, b = bf_lo(bw);
     scalars(1);
+    dc_prepare(s, s.in[0], s.prep[0], warp - 4, lane, g, b);
   } else {
     const float* st = a.state + slot * a.sS + ((long long)hv * 128 + row0 + warp * 16 + gq) * 128 + 2 * t4;
     const bool fresh = a.fresh && a.fresh[n];
@@ -247,16 +269,15 @@ __global__ void __launch_bounds__(DC_THREADS, 2) delta_chunk_kernel(DeltaArgs a)
         h[j][2 * r + 1] = x.y;
       }
   }
+  cp_async_wait<0>();
   __syncthreads();
 
   for (int c = 0; c < chunks; ++c) {
+    if (c + 2 < chunks) dc_load(a, s.in[(c + 2) % 3], t0 + (long long)(c + 2) * DC_T, e, hk, hv, row0);
+    cp_async_commit();
     if (warp >= 4) {
-      if (c + 2 < chunks) dc_load(a, s.in[(c + 2) % 3], t0 + (long long)(c + 2) * DC_T, e, hk, hv, row0, pt);
-      cp_async_commit();
       if (c + 1 < chunks) {
-        cp_async_wait<1>();
-        named_bar_sync<1, 64>();  // both warps' copies of the chunk have landed
-        const float g = gw, b = bw;
+        const float g = gw, b = bf_lo(bw);
         scalars(c + 2);
         dc_prepare(s, s.in[(c + 1) % 3], s.prep[(c + 1) & 1], warp - 4, lane, g, b);
       }
@@ -398,6 +419,7 @@ __global__ void __launch_bounds__(DC_THREADS, 2) delta_chunk_kernel(DeltaArgs a)
         }
       }
     }
+    cp_async_wait<0>();
     __syncthreads();
   }
   if (warp < 4) {

@@ -7,22 +7,29 @@
 // both running maxima, the sum and the accumulators.
 //
 // HBM-bound: every visible cache byte is read once per key/value head, for all of the head's rows together.  A CTA of four warps
-// takes 16 rows of one (sequence, head) and a chunk of its keys; each warp takes every fourth group of 16 keys, streams them
-// through its own cp.async ring (no barrier in the loop) and keeps its own softmax; the four are merged through shared memory,
+// takes 8 or 16 rows of one (sequence, head) and a chunk of its keys; each warp takes every fourth group of 16 keys, streams them
+// through its own cp.async ring (no barrier in the loop) and keeps its own sums; the four are merged through shared memory,
 // the chunks by paged_join_kernel.  A sequence that fits one chunk is written by its only CTA.
+//
+// The products are transposed, S^T = K Q^T and O^T = V^T P^T, so that keys and value columns fill the 16 rows of an m16n8k16 and
+// the 4 to 8 query rows of a decode step its 8 columns.  With query rows as the 16 (the first version of this kernel, 3.5 TB/s over
+// a long cache of head dim 256) half of the products and accumulators were padding, and 8 warps fitted an SM.
 //
 // Operands are f16: every e4m3 value is exact in f16 (cvt.rn.f16x2.e4m3x2 runs at 128 values per clock per SM, the cache
 // arrives at 22), q is scaled per row by a power of two so that its largest magnitude lies in [1, 2) (a bf16 has 8 bits, f16
-// has 11, so a value loses bits only 2^-14 below the row's largest), and p keeps f16's 11 bits.  mma.sync is right here: with 16 rows the
-// stream needs 360 of the 1024 multiply-adds per clock per SM that it sustains.
+// has 11, so a value loses bits only 2^-14 below the row's largest), and p keeps f16's 11 bits.  mma.sync is right here: the
+// stream needs 180 of the 1024 multiply-adds per clock per SM that it sustains.
 //
 // The value row's power of two cannot be applied after the product, and p * 2^nv may leave f16's range, so p's partner
-// carries it: with x_j the score in the log2 domain, P_j = 2^(x_j + nv_j - m'), m' the running maximum of x + nv, feeds the
-// product, while the sum takes 2^(x_j - m); the two maxima meet in one factor 2^(m' - m) at the end.
+// carries it: with x_j the score in the log2 domain, P_j = 2^(x_j + nv_j - m'), feeds the product, while the sum takes 2^(x_j - m);
+// the two references meet in one factor 2^(m' - m) at the end.  m and m' follow the maxima of x and x + nv lazily: they are
+// raised to the maximum only when a score passes them by more than 8 (P <= 2^8 is well within f16, and 2^-14 of the largest
+// weight still is a normal number), which one vote per 16 keys finds out.
 //
 // Fragments without shuffles: the k index of q . k may be permuted as long as q and k agree, so a thread takes 16 adjacent
 // bytes of a key row (four k16 steps at once); and ldmatrix.trans on byte pairs leaves two adjacent value columns of two keys
-// in a register, which one byte permute and two conversions turn into the fragments of the even and the odd column.
+// in a register, which one byte permute and two conversions turn into the A fragment's rows g (even column) and g + 8 (odd).
+// P^T goes from accumulator to B fragment by movmatrix.
 #pragma once
 #include <cuda_fp16.h>
 
@@ -51,13 +58,19 @@ struct PagedArgs {
   long long pages;
 };
 
-template <int D>
+// RT: groups of 8 query rows per CTA
+template <int D, int RT>
 struct PagedCfg {
-  static constexpr int WARPS = 4, STAGES = 3, KT = 16;
-  static constexpr int TILE = KT * D;                 // bytes of the K (or V) rows of one group of keys
-  static constexpr int STAGE = 2 * TILE + 48;         // + both rows of exponents, + the validity word
-  static constexpr int QBYTES = 16 * D * 2;
-  static constexpr int SMEM = QBYTES + WARPS * STAGES * STAGE;
+  static constexpr int WARPS = 4, ROWS = 8 * RT, KT = 16;
+  static constexpr int STAGES = D == 256 && RT == 1 ? 2 : 3;
+  static constexpr int CTAS = RT == 1 ? (D == 256 ? 3 : 4) : (D == 256 ? 2 : 3);  // per SM
+  static constexpr int TILE = KT * D;          // bytes of the K (or V) rows of one group of keys
+  static constexpr int STAGE = 2 * TILE + 48;  // + both rows of exponents, + the validity word
+  static constexpr int QP = 2 * D + 16;        // row pitch of q
+  static constexpr int QBYTES = ROWS * QP;
+  static constexpr int OP = D + 4;  // row pitch of a warp's merged accumulators, fp32
+  static constexpr int RING = WARPS * STAGES * STAGE, MERGE = WARPS * ROWS * OP * 4;
+  static constexpr int SMEM = QBYTES + (RING > MERGE ? RING : MERGE);
 };
 
 // 16-byte chunk of a row in shared memory.  Rows 2i and 2i + 1 must differ in bit 2 for the K reads (a quarter warp reads four
@@ -80,28 +93,40 @@ __device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr));
 }
-// Maximum of two rows' running values, -inf replaced for use as a subtrahend
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ void cp_async16_full(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// Programmatic dependent launch: the next kernel's CTAs may start once every CTA of this one has come here (or left), and
+// wait for all of this one's results at their pdl_wait.
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// A maximum for use as a subtrahend: -inf replaced
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
 
-// The keys of batch entry b that 16 rows from r0 on can see, over the sequence's own pages (positions from Lp on).
+// The keys of batch entry b that ROWS (8 or 16) rows from r0 on can see, over the sequence's own pages (positions from Lp on).
 __device__ __forceinline__ int paged_limit(const PagedArgs& a, int b, int r) {
   return r < a.M ? max(a.qpos[b * a.qpB + r / a.G], -1) - a.Lp : -1 - a.Lp;
 }
+template <int ROWS>
 __device__ __forceinline__ int paged_visible(const PagedArgs& a, int b, int r0, int lane) {
-  int lim = paged_limit(a, b, r0 + (lane & 15));
+  int lim = paged_limit(a, b, r0 + (lane & (ROWS - 1)));
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) lim = max(lim, __shfl_xor_sync(0xffffffffu, lim, o));
   return min(max(lim, -1), a.P * a.page - 1) + 1;
 }
 
-// q rows as f16 A fragments in shared memory, [D / 64][4][32 lanes] x 16 bytes: thread (g, t) of block c and word w holds rows g
-// and g + 8 at values 64 c + 16 t + 4 w .. + 3.  scale[r] takes the row's power of two out again.
-template <int D, typename RowPtr>
+// q rows as f16 in shared memory, each scaled by a power of two; srow[r] takes it out again.  128 threads, 8 per row.
+template <int D, int ROWS, int QP, typename RowPtr>
 __device__ __forceinline__ void paged_load_q(char* sq, float* srow, RowPtr row_ptr, float scale_log2) {
-  constexpr int LPR = 8;  // threads per row, 128 threads
+  constexpr int LPR = 8, V = D / (8 * LPR);  // threads per row, 16-byte loads per thread
   const int row = threadIdx.x / LPR, sub = threadIdx.x % LPR;
+  if (row >= ROWS) return;  // whole warps
   const uint16_t* p = row_ptr(row);
-  constexpr int V = D / (8 * LPR);  // 16-byte loads per thread
   uint4 x[V];
   uint32_t m = 0;
 #pragma unroll
@@ -121,26 +146,24 @@ __device__ __forceinline__ void paged_load_q(char* sq, float* srow, RowPtr row_p
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-    const int d = (i * LPR + sub) * 8;  // values d..d+3 are word w of thread t, d+4..d+7 the next word
+    uint32_t y[4];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int dd = d + 4 * k, c = dd >> 6, t = (dd >> 4) & 3, wd = (dd >> 2) & 3;
-      char* dst = sq + ((c * 4 + wd) * 32 + (row & 7) * 4 + t) * 16 + (row >> 3) * 4;
-      *reinterpret_cast<uint32_t*>(dst) = pack_f16(bf_lo(w[2 * k]) * inv, bf_hi(w[2 * k]) * inv);            // a0 / a1
-      *reinterpret_cast<uint32_t*>(dst + 8) = pack_f16(bf_lo(w[2 * k + 1]) * inv, bf_hi(w[2 * k + 1]) * inv);  // a2 / a3
-    }
+    for (int k = 0; k < 4; ++k) y[k] = pack_f16(bf_lo(w[k]) * inv, bf_hi(w[k]) * inv);
+    *reinterpret_cast<uint4*>(sq + row * QP + (i * LPR + sub) * 16) = make_uint4(y[0], y[1], y[2], y[3]);
   }
 }
 
 // Own keys (PRE = false): grid (row tiles * splits, H, B).  Prefix keys: grid (tiles of the batch's B * M rows * psplits, H).
-template <int D, bool PRE>
-__global__ void __launch_bounds__(PagedCfg<D>::WARPS * 32, D == 256 ? 2 : 3) paged_kernel(const __grid_constant__ PagedArgs a) {
-  using C = PagedCfg<D>;
+template <int D, int RT, bool PRE>
+__global__ void __launch_bounds__(128, PagedCfg<D, RT>::CTAS) paged_kernel(const __grid_constant__ PagedArgs a) {
+  using C = PagedCfg<D, RT>;
+  constexpr int ROWS = C::ROWS;
+  constexpr bool QREG = RT == 1;  // q's fragments stay in registers
   extern __shared__ __align__(128) char smem[];
-  __shared__ float srow[16];
-  __shared__ float sm[C::WARPS][3][16];
+  __shared__ float srow[ROWS];
+  __shared__ float sm[C::WARPS][3][ROWS];
   const int nsplit = PRE ? a.psplits : a.splits, chunk = PRE ? a.pchunk : a.chunk;
-  const int h = blockIdx.y, split = blockIdx.x % nsplit, r0 = blockIdx.x / nsplit * 16;
+  const int h = blockIdx.y, split = blockIdx.x % nsplit, r0 = blockIdx.x / nsplit * ROWS;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   // batch entry and row of the CTA's row i; r >= M: there is none
   auto row_of = [&](int i, int& b, int& r) {
@@ -148,10 +171,13 @@ __global__ void __launch_bounds__(PagedCfg<D>::WARPS * 32, D == 256 ? 2 : 3) pag
     r = PRE ? (r0 + i) % a.M : r0 + i;
     if (PRE && b >= a.B) b = 0, r = a.M;
   };
-  const int n = PRE ? a.Lp : paged_visible(a, blockIdx.z, r0, lane);
+  const int n = PRE ? a.Lp : paged_visible<ROWS>(a, blockIdx.z, r0, lane);
   const int c0 = split * chunk, c1 = min(n, c0 + chunk);
   const bool direct = !PRE && a.psplits == 0 && n <= chunk;  // the only chunk writes the output itself
-  if (c0 >= n && !(direct && split == 0)) return;
+  if (c0 >= n && !(direct && split == 0)) {
+    if (!PRE) pdl_wait();
+    return;
+  }
   const int ntiles = (c1 - c0 + 15) >> 4;
 
   char* ring = smem + C::QBYTES + warp * (C::STAGES * C::STAGE);
@@ -177,15 +203,24 @@ __global__ void __launch_bounds__(PagedCfg<D>::WARPS * 32, D == 256 ? 2 : 3) pag
       if (i + 1 < mine) next_id = table[group_page(i + 1, next_off)];
       const int valid = ok ? min(16, n - (c0 + (warp + C::WARPS * i) * 16)) : 0;
       const uint32_t st = ring_u + (i % C::STAGES) * C::STAGE;
-      const long long base = ok ? pid * a.cP + (long long)off * D : 0;
-      constexpr int CPR = D / 16;
+      constexpr int CPR = D / 16;  // the 16 rows are contiguous in the page
+      const long long base = (ok ? pid * a.cP + (long long)off * D : 0) + lane * 16;
+      if (valid == 16) {
 #pragma unroll
-      for (int u = 0; u < CPR / 2; ++u) {
-        const int idx = u * 32 + lane, row = idx / CPR, c = idx % CPR;
-        const uint32_t dst = st + row * D + ((c ^ paged_swz(row)) << 4);
-        const long long src = base + (row < valid ? row * D + c * 16 : 0);
-        cp_async16(dst, kb + src, row < valid);
-        cp_async16(dst + C::TILE, vb + src, row < valid);
+        for (int u = 0; u < CPR / 2; ++u) {
+          const int idx = u * 32 + lane, row = idx / CPR, c = idx % CPR;
+          const uint32_t dst = st + row * D + ((c ^ paged_swz(row)) << 4);
+          cp_async16_full(dst, kb + base + u * 512);
+          cp_async16_full(dst + C::TILE, vb + base + u * 512);
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < CPR / 2; ++u) {
+          const int idx = u * 32 + lane, row = idx / CPR, c = idx % CPR;
+          const uint32_t dst = st + row * D + ((c ^ paged_swz(row)) << 4);
+          cp_async16(dst, row < valid ? kb + base + u * 512 : kb, row < valid);
+          cp_async16(dst + C::TILE, row < valid ? vb + base + u * 512 : vb, row < valid);
+        }
       }
       if (lane < 2) {
         const long long es = ok ? pid * a.eP + off : 0;
@@ -201,29 +236,50 @@ __global__ void __launch_bounds__(PagedCfg<D>::WARPS * 32, D == 256 ? 2 : 3) pag
 #pragma unroll
   for (int i = 0; i < C::STAGES - 1; ++i) issue(i);
 
-  paged_load_q<D>(smem, srow,
-                  [&](int r) -> const uint16_t* {
-                    int b, m;
-                    row_of(r, b, m);
-                    return m < a.M ? a.q + b * a.qB + h * a.qH + m * a.qM : nullptr;
-                  },
-                  a.scale_log2);
+  paged_load_q<D, ROWS, C::QP>(smem, srow,
+                               [&](int r) -> const uint16_t* {
+                                 int b, m;
+                                 row_of(r, b, m);
+                                 return m < a.M ? a.q + b * a.qB + h * a.qH + m * a.qM : nullptr;
+                               },
+                               a.scale_log2);
   __syncthreads();
-  int lim[2];
+  int lim[RT][2];  // rows 8 rt + 2 t, + 1
+  float rs[RT][2];
+  int least = 0x7fffffff;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    int b, m;
-    row_of(g + 8 * i, b, m);
-    lim[i] = paged_limit(a, b, m) + (PRE ? a.Lp : 0);
+  for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      int b, m;
+      row_of(rt * 8 + 2 * t + e, b, m);
+      // rows past M see what there is, so that they do not make every group of keys a masked one
+      lim[rt][e] = m < a.M ? min(paged_limit(a, b, m) + (PRE ? a.Lp : 0), n - 1) : n - 1;
+      rs[rt][e] = srow[rt * 8 + 2 * t + e];
+      least = min(least, lim[rt][e]);
+    }
+  // q's B fragments: thread (g, t) holds row g at 64 c + 16 t .. + 15, the k16 steps' words w at + 4 w
+  uint4 qf[QREG ? D / 64 : 1][2];
+  const char* qrow = smem + g * C::QP + t * 32;
+  if (QREG) {
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) qf[c][x] = *reinterpret_cast<const uint4*>(qrow + c * 128 + x * 16);
   }
-  const float rs[2] = {srow[g], srow[g + 8]};
 
-  float o[D / 16][2][4];
+  float o[RT][D / 16][4];
+  float m[RT][2], mv[RT][2], l[RT][2];
 #pragma unroll
-  for (int j = 0; j < D / 16; ++j)
+  for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[j][0][e] = o[j][1][e] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, mv[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[rt][j][e] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) m[rt][e] = mv[rt][e] = -INFINITY, l[rt][e] = 0.f;
+  }
+  const uint32_t vofs = C::TILE + (lane & 15) * D;
 
   for (int i = 0; i < mine; ++i) {
     issue(i + C::STAGES - 1);
@@ -231,84 +287,105 @@ __global__ void __launch_bounds__(PagedCfg<D>::WARPS * 32, D == 256 ? 2 : 3) pag
     __syncwarp();
     const int j0 = c0 + (warp + C::WARPS * i) * 16;
     const char* st = ring + (i % C::STAGES) * C::STAGE;
-    // ---- scores of 16 keys: two n8 tiles, two chains of k steps each
-    float s[2][2][4];
+    // ---- scores: 16 keys x 8 rows, two chains of k steps
+    float s[RT][2][4];
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt)
+    for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[nt][0][e] = s[nt][1][e] = 0.f;
+      for (int e = 0; e < 4; ++e) s[rt][0][e] = s[rt][1][e] = 0.f;
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) {
-      uint4 kx[2];
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
-        kx[nt] = *reinterpret_cast<const uint4*>(st + (nt * 8 + g) * D + (((c * 4 + t) ^ paged_swz(g)) << 4));
+      const uint4 k0 = *reinterpret_cast<const uint4*>(st + g * D + (((c * 4 + t) ^ paged_swz(g)) << 4));
+      const uint4 k1 = *reinterpret_cast<const uint4*>(st + (g + 8) * D + (((c * 4 + t) ^ paged_swz(g)) << 4));
+      const uint32_t kw0[4] = {k0.x, k0.y, k0.z, k0.w}, kw1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const uint4 qx = *reinterpret_cast<const uint4*>(smem + ((c * 4 + w) * 32 + lane) * 16);
-        const uint32_t qa[4] = {qx.x, qx.y, qx.z, qx.w};
+        const uint32_t ka[4] = {e4m3x2_f16x2((uint16_t)kw0[w]), e4m3x2_f16x2((uint16_t)kw1[w]),
+                                e4m3x2_f16x2((uint16_t)(kw0[w] >> 16)), e4m3x2_f16x2((uint16_t)(kw1[w] >> 16))};
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          const uint32_t kw = w == 0 ? kx[nt].x : w == 1 ? kx[nt].y : w == 2 ? kx[nt].z : kx[nt].w;
-          mma_f16(s[nt][w & 1], qa, e4m3x2_f16x2((uint16_t)kw), e4m3x2_f16x2((uint16_t)(kw >> 16)));
+        for (int rt = 0; rt < RT; ++rt) {
+          const uint4 q4 = QREG ? qf[QREG ? c : 0][w >> 1]
+                                : *reinterpret_cast<const uint4*>(qrow + rt * 8 * C::QP + c * 128 + (w >> 1) * 16);
+          mma_f16(s[rt][w & 1], ka, w & 1 ? q4.z : q4.x, w & 1 ? q4.w : q4.y);
         }
       }
     }
-    // ---- scale, mask, both maxima
-    const bool ok = *reinterpret_cast<const int*>(st + 2 * C::TILE + 32);
-    float x[2][2][2], nv[2][2];
-#pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
-      const uint32_t ek = *reinterpret_cast<const uint16_t*>(st + 2 * C::TILE + nt * 8 + 2 * t);
-      const uint32_t ev = *reinterpret_cast<const uint16_t*>(st + 2 * C::TILE + 16 + nt * 8 + 2 * t);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float ks = pow2_byte((ek >> (8 * e)) & 255u);
-        const uint32_t vbyte = (ev >> (8 * e)) & 255u;
-        nv[nt][e] = vbyte == 255u ? __uint_as_float(0x7fc00000u) : (float)((int)vbyte - 127);
-        const int j = j0 + nt * 8 + 2 * t + e;
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-          x[r][nt][e] = ok && j <= lim[r] && j < n ? (s[nt][0][2 * r + e] + s[nt][1][2 * r + e]) * (rs[r] * ks) : -INFINITY;
-      }
-    }
-    float alpha[2];
-    uint32_t pa[4];
-    bool grew = false;
+    // ---- scale, mask; the keys of a thread are g and g + 8
+    const char* meta = st + 2 * C::TILE;
+    const float ks[2] = {pow2_byte((uint8_t)meta[g]), pow2_byte((uint8_t)meta[g + 8])};
+    float nv[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      float mx = fmaxf(fmaxf(x[r][0][0], x[r][0][1]), fmaxf(x[r][1][0], x[r][1][1]));
-      float my = fmaxf(fmaxf(x[r][0][0] + nv[0][0], x[r][0][1] + nv[0][1]), fmaxf(x[r][1][0] + nv[1][0], x[r][1][1] + nv[1][1]));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      my = fmaxf(my, __shfl_xor_sync(0xffffffffu, my, 1));
-      mx = fmaxf(m[r], fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)));
-      my = fmaxf(mv[r], fmaxf(my, __shfl_xor_sync(0xffffffffu, my, 2)));
-      grew |= my != mv[r];
-      const float ux = finite_or_zero(mx), uy = finite_or_zero(my);
-      l[r] *= ex2_approx(m[r] - ux);
-      alpha[r] = ex2_approx(mv[r] - uy);
-      m[r] = mx;
-      mv[r] = my;
+      const int vbyte = (uint8_t)meta[16 + g + 8 * r];
+      nv[r] = vbyte == 255 ? __uint_as_float(0x7fc00000u) : (float)(vbyte - 127);
+    }
+    float x[RT][2][2], y[RT][2][2];  // [key][row]
+    bool over = false;
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        l[r] += ex2_approx(x[r][nt][0] - ux) + ex2_approx(x[r][nt][1] - ux);
-        // a masked key's exponent may be any byte, NaN's too: its weight is 0, not 2^NaN
-        const float p0 = x[r][nt][0] == -INFINITY ? 0.f : ex2_approx(x[r][nt][0] + nv[nt][0] - uy);
-        const float p1 = x[r][nt][1] == -INFINITY ? 0.f : ex2_approx(x[r][nt][1] + nv[nt][1] - uy);
-        pa[nt * 2 + r] = pack_f16(p0, p1);
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) x[rt][r][e] = (s[rt][0][2 * r + e] + s[rt][1][2 * r + e]) * (rs[rt][e] * ks[r]);
+    if (__any_sync(0xffffffffu, j0 + 15 > least) || !*reinterpret_cast<const int*>(meta + 32)) {
+      const bool ok = *reinterpret_cast<const int*>(meta + 32);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+            if (!ok || j0 + g + 8 * r > lim[rt][e]) x[rt][r][e] = -INFINITY;
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          // a masked key's exponent may be any byte, NaN's too
+          y[rt][r][e] = x[rt][r][e] == -INFINITY ? -INFINITY : x[rt][r][e] + nv[r];
+          over |= x[rt][r][e] > m[rt][e] + 8.f || y[rt][r][e] > mv[rt][e] + 8.f;
+        }
+    if (__any_sync(0xffffffffu, over)) {  // raise the references to the maxima
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        float al[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float mx = fmaxf(x[rt][0][e], x[rt][1][e]), my = fmaxf(y[rt][0][e], y[rt][1][e]);
+#pragma unroll
+          for (int k = 4; k < 32; k <<= 1) {
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
+            my = fmaxf(my, __shfl_xor_sync(0xffffffffu, my, k));
+          }
+          mx = fmaxf(mx, m[rt][e]);
+          my = fmaxf(my, mv[rt][e]);
+          l[rt][e] *= ex2_approx(m[rt][e] - finite_or_zero(mx));
+          al[e] = ex2_approx(mv[rt][e] - finite_or_zero(my));
+          m[rt][e] = mx;
+          mv[rt][e] = my;
+        }
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[rt][j][e] *= al[e & 1];
       }
     }
-    if (__any_sync(0xffffffffu, grew)) {
+    uint32_t pb[RT][2];
 #pragma unroll
-      for (int j = 0; j < D / 16; ++j)
+    for (int rt = 0; rt < RT; ++rt) {
+      const float u[2] = {finite_or_zero(m[rt][0]), finite_or_zero(m[rt][1])};
+      const float uv[2] = {finite_or_zero(mv[rt][0]), finite_or_zero(mv[rt][1])};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          o[j][0][e] *= alpha[e >> 1];
-          o[j][1][e] *= alpha[e >> 1];
-        }
+      for (int r = 0; r < 2; ++r) {
+        l[rt][0] += ex2_approx(x[rt][r][0] - u[0]);
+        l[rt][1] += ex2_approx(x[rt][r][1] - u[1]);
+        pb[rt][r] = movmatrix(pack_f16(ex2_approx(y[rt][r][0] - uv[0]), ex2_approx(y[rt][r][1] - uv[1])));
+      }
     }
-    // ---- o += P V
-    const uint32_t vrow = ring_u + (i % C::STAGES) * C::STAGE + C::TILE + (lane & 15) * D;
+    // ---- o^T += V^T P^T
+    const uint32_t vrow = ring_u + (i % C::STAGES) * C::STAGE + vofs;
 #pragma unroll
     for (int j = 0; j < D / 16; j += 2) {
       uint32_t v4[4];
@@ -316,42 +393,54 @@ __global__ void __launch_bounds__(PagedCfg<D>::WARPS * 32, D == 256 ? 2 : 3) pag
 #pragma unroll
       for (int jj = 0; jj < 2; ++jj) {
         const uint32_t lo = __byte_perm(v4[2 * jj], 0, 0x3120), hi = __byte_perm(v4[2 * jj + 1], 0, 0x3120);
-        mma_f16(o[j + jj][0], pa, e4m3x2_f16x2((uint16_t)lo), e4m3x2_f16x2((uint16_t)hi));
-        mma_f16(o[j + jj][1], pa, e4m3x2_f16x2((uint16_t)(lo >> 16)), e4m3x2_f16x2((uint16_t)(hi >> 16)));
+        const uint32_t va[4] = {e4m3x2_f16x2((uint16_t)lo), e4m3x2_f16x2((uint16_t)(lo >> 16)), e4m3x2_f16x2((uint16_t)hi),
+                                e4m3x2_f16x2((uint16_t)(hi >> 16))};
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) mma_f16(o[rt][j + jj], va, pb[rt][0], pb[rt][1]);
       }
     }
     __syncwarp();  // the stage may be filled again
   }
   cp_async_wait<0>();
+  pdl_launch();
 
   // ---- merge the four warps
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    if (t == 0) {
-      sm[warp][0][g + 8 * r] = m[r];
-      sm[warp][1][g + 8 * r] = mv[r];
-      sm[warp][2][g + 8 * r] = l[r];
+  for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int k = 4; k < 32; k <<= 1) l[rt][e] += __shfl_xor_sync(0xffffffffu, l[rt][e], k);
+      if (g == 0) {
+        const int r = rt * 8 + 2 * t + e;
+        sm[warp][0][r] = m[rt][e];
+        sm[warp][1][r] = mv[rt][e];
+        sm[warp][2][r] = l[rt][e];
+      }
     }
-  }
-  __syncthreads();  // all rings are drained: their space takes the accumulators, [warp][16][D + 4] fp32
-  constexpr int OP = D + 4;
-  float* so = reinterpret_cast<float*>(smem);
-  static_assert(C::WARPS * 16 * OP * 4 <= C::SMEM, "the accumulators fit the ring");
+  __syncthreads();  // all rings are drained: their space takes the accumulators, [warp][ROWS][OP] fp32
+  float* so = reinterpret_cast<float*>(smem + C::QBYTES);
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    float top = -INFINITY;
+  for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-    for (int w = 0; w < C::WARPS; ++w) top = fmaxf(top, sm[w][1][g + 8 * r]);
-    const float f = ex2_approx(mv[r] - finite_or_zero(top));
+    for (int e = 0; e < 2; ++e) {
+      const int r = rt * 8 + 2 * t + e;
+      float top = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < D / 16; ++j)
-      *reinterpret_cast<float4*>(so + (warp * 16 + g + 8 * r) * OP + 16 * j + 4 * t) =
-          make_float4(o[j][0][2 * r] * f, o[j][1][2 * r] * f, o[j][0][2 * r + 1] * f, o[j][1][2 * r + 1] * f);
-  }
+      for (int w = 0; w < C::WARPS; ++w) top = fmaxf(top, sm[w][1][r]);
+      const float f = ex2_approx(mv[rt][e] - finite_or_zero(top));
+      // value columns 16 j + 2 g, + 1 (a NaN weight stays NaN; a warp without visible keys adds zeros)
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j)
+        *reinterpret_cast<float2*>(so + (warp * ROWS + r) * C::OP + 16 * j + 2 * g) =
+            make_float2(o[rt][j][e] * f, o[rt][j][2 + e] * f);
+    }
   __syncthreads();
+  // The own keys' kernel runs beside the prefix's (none of its inputs come from there), and ends after it: so what is launched
+  // behind it finds both results
+  if (!PRE) pdl_wait();
   const int row = threadIdx.x >> 3, sub = threadIdx.x & 7;  // 8 threads a row
+  if (row >= ROWS) return;
   int b, mr;
   row_of(row, b, mr);
   if (mr >= a.M) return;
@@ -371,7 +460,7 @@ __global__ void __launch_bounds__(PagedCfg<D>::WARPS * 32, D == 256 ? 2 : 3) pag
     for (int e = 0; e < 8; ++e) {
       v[e] = 0.f;
 #pragma unroll
-      for (int w = 0; w < C::WARPS; ++w) v[e] += so[(w * 16 + row) * OP + d + e];
+      for (int w = 0; w < C::WARPS; ++w) v[e] += so[(w * ROWS + row) * C::OP + d + e];
       v[e] = sum == 0.f ? 0.f : v[e] * fac;
     }
     if (direct) {
@@ -386,17 +475,21 @@ __global__ void __launch_bounds__(PagedCfg<D>::WARPS * 32, D == 256 ? 2 : 3) pag
   if (!direct && sub == 0) a.lse[at] = sum == 0.f ? -INFINITY : top + log2f(sum);
 }
 
-// Joins the chunks' partial outputs: one warp per row.
-template <int D>
+// Joins the chunks' partial outputs: one warp per row; ROWS: rows per CTA of the launch that made them.
+template <int D, int ROWS>
 __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedArgs a) {
   const int lane = threadIdx.x & 31;
   const long long rows = (long long)a.B * a.H * a.M, R = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (R >= rows) return;
   const int r = (int)(R % a.M), h = (int)(R / a.M % a.H), b = (int)(R / a.M / a.H);
-  const int n = paged_visible(a, b, r & ~15, lane);
-  if (a.psplits == 0 && n <= a.chunk) return;  // written by its only chunk
+  const int n = paged_visible<ROWS>(a, b, r & ~(ROWS - 1), lane);
+  if (a.psplits == 0 && n <= a.chunk) {  // written by its only chunk
+    pdl_wait();
+    return;
+  }
   const int mine = (n + a.chunk - 1) / a.chunk, total = mine + a.psplits;
   auto slot = [&](int i) { return i < mine ? i : a.splits + i - mine; };
+  pdl_wait();
   float top = -INFINITY;
   bool nan = false;
   for (int i = lane; i < total; i += 32) {
@@ -446,17 +539,17 @@ inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 // many CTAs as keep every SM at its resident count about three times over when all sequences are full, but no chunk under 256
 // keys, 64 for each of the four warps.
 inline PagedPlan paged_plan(int B, int H, int M, int D, int P, int page, int Lp, int sms) {
-  const int resident = D == 256 ? 2 : 3;
-  auto cut = [&](long long keys, long long units, int& chunk, int& splits) {
+  auto cut = [&](long long keys, long long units, int resident, int& chunk, int& splits) {
     const long long want = (3LL * sms * resident + units - 1) / units;
     long long c = (keys + want - 1) / want;
     c = (c + 63) / 64 * 64;
     chunk = (int)(c < 256 ? 256 : c);
     splits = keys ? ceil_div(keys, chunk) : 0;
   };
+  const int rows = M <= 8 ? 8 : 16, resident = M <= 8 ? (D == 256 ? 3 : 4) : (D == 256 ? 2 : 3);
   PagedPlan p;
-  cut((long long)P * page, (long long)B * H * ceil_div(M, 16), p.chunk, p.splits);
-  cut(Lp, (long long)H * ceil_div((long long)B * M, 16), p.pchunk, p.psplits);
+  cut((long long)P * page, (long long)B * H * ceil_div(M, rows), resident, p.chunk, p.splits);
+  cut(Lp, (long long)H * ceil_div((long long)B * M, 16), D == 256 ? 2 : 3, p.pchunk, p.psplits);
   if (p.splits == 0) p.splits = 1;  // no pages at all: one chunk without keys
   return p;
 }
@@ -469,22 +562,43 @@ inline int paged_check(int B, int H, int M, int G, int D, int P, int page, int L
   return 0;
 }
 
+// One launch of 128 threads a CTA; dependent: as a programmatic dependent of the launch before it
+inline int launch_dependent(void (*kernel)(const reax::PagedArgs), dim3 grid, int smem, bool dependent, const reax::PagedArgs& a,
+                            cudaStream_t st) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = dependent ? 1 : 0;
+  return (int)cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+template <int D, int RT, bool PRE>
+inline int paged_launch(const reax::PagedArgs& a, cudaStream_t st) {
+  using C = reax::PagedCfg<D, RT>;
+  static SmemAttr attr;
+  if (ensure_smem(attr, reax::paged_kernel<D, RT, PRE>, C::SMEM, true) != cudaSuccess) return -4;
+  const long long x = PRE ? (long long)ceil_div((long long)a.B * a.M, C::ROWS) * a.psplits : (long long)ceil_div(a.M, C::ROWS) * a.splits;
+  if (x > 0x7fffffffLL) return -1;
+  return launch_dependent(reax::paged_kernel<D, RT, PRE>, dim3((unsigned)x, a.H, PRE ? 1 : a.B), C::SMEM, !PRE && a.psplits, a, st);
+}
+
+// Up to 8 rows per (sequence, head), what a decode step has, go in one group of 8; more in CTAs of 16 rows.
 template <int D>
 inline int paged_go(const reax::PagedArgs& a, cudaStream_t st) {
-  using C = reax::PagedCfg<D>;
-  static SmemAttr own, pre;
-  if (ensure_smem(own, reax::paged_kernel<D, false>, C::SMEM, true) != cudaSuccess) return -4;
-  if (ensure_smem(pre, reax::paged_kernel<D, true>, C::SMEM, true) != cudaSuccess) return -4;
-  const long long tiles = ceil_div(a.M, 16), ptiles = ceil_div((long long)a.B * a.M, 16);
-  if (tiles * a.splits > 0x7fffffffLL || ptiles * a.psplits > 0x7fffffffLL) return -1;
   if (a.psplits)
-    reax::paged_kernel<D, true><<<dim3((unsigned)(ptiles * a.psplits), a.H), C::WARPS * 32, C::SMEM, st>>>(a);
-  reax::paged_kernel<D, false><<<dim3((unsigned)(tiles * a.splits), a.H, a.B), C::WARPS * 32, C::SMEM, st>>>(a);
+    if (int rc = paged_launch<D, 2, true>(a, st)) return rc;
+  if (int rc = a.M <= 8 ? paged_launch<D, 1, false>(a, st) : paged_launch<D, 2, false>(a, st)) return rc;
   if (a.splits + a.psplits > 1) {
-    const long long rows = (long long)a.B * a.H * a.M;
-    reax::paged_join_kernel<D><<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(a);
+    const unsigned x = (unsigned)(((long long)a.B * a.H * a.M + 3) / 4);
+    return launch_dependent(a.M <= 8 ? reax::paged_join_kernel<D, 8> : reax::paged_join_kernel<D, 16>, dim3(x), 0, true, a, st);
   }
-  return (int)cudaGetLastError();
+  return 0;
 }
 
 }  // namespace reax_host
