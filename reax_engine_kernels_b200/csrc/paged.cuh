@@ -27,8 +27,8 @@
 // weight still is a normal number), which one vote per 16 keys finds out.
 //
 // Fragments without shuffles: the k index of q . k may be permuted as long as q and k agree, so a thread takes 16 adjacent
-// bytes of a key row (four k16 steps at once); and ldmatrix.trans on byte pairs leaves two adjacent value columns of two keys
-// in a register, which one byte permute and two conversions turn into the A fragment's rows g (even column) and g + 8 (odd).
+// bytes of a key row (four k16 steps at once).  ldmatrix.m16n16.trans.b8 leaves four consecutive keys of a value column in a register,
+// so the keys' order in P V is made to suit: row g of S^T is key 4 (g / 2) + g % 2 of its 16, row g + 8 the key two behind it.
 // P^T goes from accumulator to B fragment by movmatrix.
 #pragma once
 #include <cuda_fp16.h>
@@ -73,8 +73,8 @@ struct PagedCfg {
   static constexpr int SMEM = QBYTES + (RING > MERGE ? RING : MERGE);
 };
 
-// 16-byte chunk of a row in shared memory.  Rows 2i and 2i + 1 must differ in bit 2 for the K reads (a quarter warp reads four
-// chunks of each), all eight rows of a group for ldmatrix.
+// 16-byte chunk of a row in shared memory.  Rows 4i and 4i + 1 (and the two behind them) must differ in bit 2 for the K reads (a
+// quarter warp reads four chunks of each), all rows of a group of eight for ldmatrix.
 __device__ __forceinline__ int paged_swz(int row) { return ((row & 1) << 2) | ((row >> 1) & 3); }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -88,8 +88,10 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+// two 16 x 16 byte matrices (rows: lanes 0-15, 16-31), transposed: r[2 i] holds bytes 4 t .. + 3 of column g of the i-th, r[2 i + 1]
+// of column g + 8
+__device__ __forceinline__ void ldsm_b8_x2_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr));
 }
@@ -279,14 +281,22 @@ __global__ void __launch_bounds__(128, PagedCfg<D, RT>::CTAS) paged_kernel(const
 #pragma unroll
     for (int e = 0; e < 2; ++e) m[rt][e] = mv[rt][e] = -INFINITY, l[rt][e] = 0.f;
   }
-  const uint32_t vofs = C::TILE + (lane & 15) * D;
+  const int key = 4 * (g >> 1) + (g & 1);  // this thread's keys: key and key + 2
+  // A row's chunk c ^ swz: the part of c that the unrolled loops count stays out of the XOR
+  const int ksw = (t ^ (paged_swz(key) & 3)) << 4, kbit = (paged_swz(key) & 4) << 4;
+  const int ksw2 = (t ^ (paged_swz(key + 2) & 3)) << 4, kbit2 = (paged_swz(key + 2) & 4) << 4;
+  const int vrow = lane & 15, vsw = (lane >> 4) ^ paged_swz(vrow);
+  int slot = 0;
 
   for (int i = 0; i < mine; ++i) {
     issue(i + C::STAGES - 1);
     cp_async_wait<C::STAGES - 1>();
     __syncwarp();
     const int j0 = c0 + (warp + C::WARPS * i) * 16;
-    const char* st = ring + (i % C::STAGES) * C::STAGE;
+    const char* st = ring + slot * C::STAGE;
+    const char *kr0 = st + key * D + ksw, *kr1 = st + (key + 2) * D + ksw2;
+    const uint32_t vr = ring_u + slot * C::STAGE + C::TILE + vrow * D;
+    slot = slot + 1 == C::STAGES ? 0 : slot + 1;
     // ---- scores: 16 keys x 8 rows, two chains of k steps
     float s[RT][2][4];
 #pragma unroll
@@ -295,8 +305,8 @@ __global__ void __launch_bounds__(128, PagedCfg<D, RT>::CTAS) paged_kernel(const
       for (int e = 0; e < 4; ++e) s[rt][0][e] = s[rt][1][e] = 0.f;
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) {
-      const uint4 k0 = *reinterpret_cast<const uint4*>(st + g * D + (((c * 4 + t) ^ paged_swz(g)) << 4));
-      const uint4 k1 = *reinterpret_cast<const uint4*>(st + (g + 8) * D + (((c * 4 + t) ^ paged_swz(g)) << 4));
+      const uint4 k0 = *reinterpret_cast<const uint4*>(kr0 + ((c * 64) ^ kbit));
+      const uint4 k1 = *reinterpret_cast<const uint4*>(kr1 + ((c * 64) ^ kbit2));
       const uint32_t kw0[4] = {k0.x, k0.y, k0.z, k0.w}, kw1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
@@ -310,13 +320,13 @@ __global__ void __launch_bounds__(128, PagedCfg<D, RT>::CTAS) paged_kernel(const
         }
       }
     }
-    // ---- scale, mask; the keys of a thread are g and g + 8
+    // ---- scale, mask
     const char* meta = st + 2 * C::TILE;
-    const float ks[2] = {pow2_byte((uint8_t)meta[g]), pow2_byte((uint8_t)meta[g + 8])};
+    const float ks[2] = {pow2_byte((uint8_t)meta[key]), pow2_byte((uint8_t)meta[key + 2])};
     float nv[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int vbyte = (uint8_t)meta[16 + g + 8 * r];
+      const int vbyte = (uint8_t)meta[16 + key + 2 * r];
       nv[r] = vbyte == 255 ? __uint_as_float(0x7fc00000u) : (float)(vbyte - 127);
     }
     float x[RT][2][2], y[RT][2][2];  // [key][row]
@@ -335,7 +345,7 @@ __global__ void __launch_bounds__(128, PagedCfg<D, RT>::CTAS) paged_kernel(const
         for (int e = 0; e < 2; ++e)
 #pragma unroll
           for (int r = 0; r < 2; ++r)
-            if (!ok || j0 + g + 8 * r > lim[rt][e]) x[rt][r][e] = -INFINITY;
+            if (!ok || j0 + key + 2 * r > lim[rt][e]) x[rt][r][e] = -INFINITY;
     }
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
@@ -385,16 +395,14 @@ __global__ void __launch_bounds__(128, PagedCfg<D, RT>::CTAS) paged_kernel(const
       }
     }
     // ---- o^T += V^T P^T
-    const uint32_t vrow = ring_u + (i % C::STAGES) * C::STAGE + vofs;
 #pragma unroll
     for (int j = 0; j < D / 16; j += 2) {
       uint32_t v4[4];
-      ldsm_x4_trans(vrow + (((j + (lane >> 4)) ^ paged_swz(lane & 7)) << 4), v4);
+      ldsm_b8_x2_trans(vr + ((j ^ vsw) << 4), v4);
 #pragma unroll
       for (int jj = 0; jj < 2; ++jj) {
-        const uint32_t lo = __byte_perm(v4[2 * jj], 0, 0x3120), hi = __byte_perm(v4[2 * jj + 1], 0, 0x3120);
-        const uint32_t va[4] = {e4m3x2_f16x2((uint16_t)lo), e4m3x2_f16x2((uint16_t)(lo >> 16)), e4m3x2_f16x2((uint16_t)hi),
-                                e4m3x2_f16x2((uint16_t)(hi >> 16))};
+        const uint32_t va[4] = {e4m3x2_f16x2((uint16_t)v4[2 * jj]), e4m3x2_f16x2((uint16_t)v4[2 * jj + 1]),
+                                e4m3x2_f16x2((uint16_t)(v4[2 * jj] >> 16)), e4m3x2_f16x2((uint16_t)(v4[2 * jj + 1] >> 16))};
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) mma_f16(o[rt][j + jj], va, pb[rt][0], pb[rt][1]);
       }
@@ -429,11 +437,12 @@ __global__ void __launch_bounds__(128, PagedCfg<D, RT>::CTAS) paged_kernel(const
 #pragma unroll
       for (int w = 0; w < C::WARPS; ++w) top = fmaxf(top, sm[w][1][r]);
       const float f = ex2_approx(mv[rt][e] - finite_or_zero(top));
-      // value columns 16 j + 2 g, + 1 (a NaN weight stays NaN; a warp without visible keys adds zeros)
+      // a NaN weight stays NaN; a warp without visible keys adds zeros
 #pragma unroll
-      for (int j = 0; j < D / 16; ++j)
-        *reinterpret_cast<float2*>(so + (warp * ROWS + r) * C::OP + 16 * j + 2 * g) =
-            make_float2(o[rt][j][e] * f, o[rt][j][2 + e] * f);
+      for (int j = 0; j < D / 16; ++j) {
+        so[(warp * ROWS + r) * C::OP + 16 * j + g] = o[rt][j][e] * f;
+        so[(warp * ROWS + r) * C::OP + 16 * j + 8 + g] = o[rt][j][2 + e] * f;
+      }
     }
   __syncthreads();
   // The own keys' kernel runs beside the prefix's (none of its inputs come from there), and ends after it: so what is launched
@@ -475,55 +484,58 @@ __global__ void __launch_bounds__(128, PagedCfg<D, RT>::CTAS) paged_kernel(const
   if (!direct && sub == 0) a.lse[at] = sum == 0.f ? -INFINITY : top + log2f(sum);
 }
 
-// Joins the chunks' partial outputs: one warp per row; ROWS: rows per CTA of the launch that made them.
+// Joins the chunks' partial outputs: one CTA per row; D / 4 threads take four values each, 128 / (D / 4) groups of them every other
+// chunk.  ROWS: rows per CTA of the launch that made them.
 template <int D, int ROWS>
 __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedArgs a) {
-  const int lane = threadIdx.x & 31;
-  const long long rows = (long long)a.B * a.H * a.M, R = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (R >= rows) return;
+  constexpr int TPG = D / 4, GROUPS = 128 / TPG;
+  __shared__ float red[4], sum_s[GROUPS];
+  __shared__ __align__(16) float acc_s[GROUPS][D];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, grp = threadIdx.x / TPG, d = threadIdx.x % TPG * 4;
+  const long long rows = (long long)a.B * a.H * a.M, R = blockIdx.x;
   const int r = (int)(R % a.M), h = (int)(R / a.M % a.H), b = (int)(R / a.M / a.H);
   const int n = paged_visible<ROWS>(a, b, r & ~(ROWS - 1), lane);
-  if (a.psplits == 0 && n <= a.chunk) {  // written by its only chunk
-    pdl_wait();
-    return;
-  }
-  const int mine = (n + a.chunk - 1) / a.chunk, total = mine + a.psplits;
-  auto slot = [&](int i) { return i < mine ? i : a.splits + i - mine; };
   pdl_wait();
+  if (a.psplits == 0 && n <= a.chunk) return;  // written by its only chunk
+  const int mine = (n + a.chunk - 1) / a.chunk, total = mine + a.psplits;
+  auto slot = [&](int i) { return (i < mine ? i : a.splits + i - mine) * rows + R; };
   float top = -INFINITY;
   bool nan = false;
-  for (int i = lane; i < total; i += 32) {
-    const float x = a.lse[slot(i) * rows + R];
+  for (int i = threadIdx.x; i < total; i += 128) {
+    const float x = a.lse[slot(i)];
     nan |= x != x;
     top = fmaxf(top, x);
   }
 #pragma unroll
   for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-  if (__any_sync(0xffffffffu, nan)) top = __uint_as_float(0x7fc00000u);
-  const float ref = finite_or_zero(top);
-  constexpr int V = D / 32;
-  float acc[V], sum = 0.f;
-#pragma unroll
-  for (int e = 0; e < V; ++e) acc[e] = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < total; ++i) {
-    const long long at = slot(i) * rows + R;
+  if (lane == 0) red[warp] = top;
+  nan = __syncthreads_or(nan);
+  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float ref = nan ? __uint_as_float(0x7fc00000u) : finite_or_zero(top);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+#pragma unroll 8
+  for (int i = grp; i < total; i += GROUPS) {
+    const long long at = slot(i);
     const float w = ex2_approx(a.lse[at] - ref);
+    const float4 x = *reinterpret_cast<const float4*>(a.part + at * D + d);
     sum += w;
-    const float4* p = reinterpret_cast<const float4*>(a.part + at * D + lane * V);
+    acc.x += w * x.x, acc.y += w * x.y, acc.z += w * x.z, acc.w += w * x.w;
+  }
+  *reinterpret_cast<float4*>(&acc_s[grp][d]) = acc;
+  if (threadIdx.x % TPG == 0) sum_s[grp] = sum;
+  __syncthreads();
+  if (grp) return;
+  sum = sum_s[0];
 #pragma unroll
-    for (int e = 0; e < V / 4; ++e) {
-      const float4 x = p[e];
-      acc[4 * e] += w * x.x, acc[4 * e + 1] += w * x.y, acc[4 * e + 2] += w * x.z, acc[4 * e + 3] += w * x.w;
-    }
+  for (int i = 1; i < GROUPS; ++i) {
+    const float4 x = *reinterpret_cast<const float4*>(&acc_s[i][d]);
+    acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
+    sum += sum_s[i];
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  uint32_t y[V / 2];
-#pragma unroll
-  for (int e = 0; e < V / 2; ++e) y[e] = pack_bf16(acc[2 * e] * inv, acc[2 * e + 1] * inv);
-  uint16_t* out = a.o + b * a.oB + h * a.oH + r * a.oM + lane * V;
-  if (V == 8) *reinterpret_cast<uint4*>(out) = make_uint4(y[0], y[1], y[V / 2 - 2], y[V / 2 - 1]);
-  else *reinterpret_cast<uint2*>(out) = make_uint2(y[0], y[1]);
+  *reinterpret_cast<uint2*>(a.o + b * a.oB + h * a.oH + r * a.oM + d) =
+      make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
 }
 
 }  // namespace reax
@@ -540,10 +552,16 @@ inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 // keys, 64 for each of the four warps.
 inline PagedPlan paged_plan(int B, int H, int M, int D, int P, int page, int Lp, int sms) {
   auto cut = [&](long long keys, long long units, int resident, int& chunk, int& splits) {
-    const long long want = (3LL * sms * resident + units - 1) / units;
+    #ifndef PW
+#define PW 3LL
+#endif
+    const long long want = (PW * sms * resident + units - 1) / units;
     long long c = (keys + want - 1) / want;
     c = (c + 63) / 64 * 64;
-    chunk = (int)(c < 256 ? 256 : c);
+    #ifndef PMIN
+#define PMIN 256
+#endif
+    chunk = (int)(c < PMIN ? PMIN : c);
     splits = keys ? ceil_div(keys, chunk) : 0;
   };
   const int rows = M <= 8 ? 8 : 16, resident = M <= 8 ? (D == 256 ? 3 : 4) : (D == 256 ? 2 : 3);
@@ -558,7 +576,8 @@ inline int paged_check(int B, int H, int M, int G, int D, int P, int page, int L
   if (D != 128 && D != 256) return -3;
   if (page <= 0 || page % 16) return -2;
   if (B < 0 || B > 65535 || H <= 0 || H > 65535 || M < 0 || G <= 0 || P < 0 || Lp < 0) return -1;
-  if ((long long)P * page > (1LL << 30) || Lp > (1 << 30) || (long long)B * M > (1LL << 30)) return -1;
+  if ((long long)P * page > (1LL << 30) || Lp > (1 << 30) || (long long)B * M > (1LL << 30) || (long long)B * H * M > 0x7fffffffLL)
+    return -1;
   return 0;
 }
 
@@ -595,8 +614,8 @@ inline int paged_go(const reax::PagedArgs& a, cudaStream_t st) {
     if (int rc = paged_launch<D, 2, true>(a, st)) return rc;
   if (int rc = a.M <= 8 ? paged_launch<D, 1, false>(a, st) : paged_launch<D, 2, false>(a, st)) return rc;
   if (a.splits + a.psplits > 1) {
-    const unsigned x = (unsigned)(((long long)a.B * a.H * a.M + 3) / 4);
-    return launch_dependent(a.M <= 8 ? reax::paged_join_kernel<D, 8> : reax::paged_join_kernel<D, 16>, dim3(x), 0, true, a, st);
+    const dim3 rows((unsigned)((long long)a.B * a.H * a.M));
+    return launch_dependent(a.M <= 8 ? reax::paged_join_kernel<D, 8> : reax::paged_join_kernel<D, 16>, rows, 0, true, a, st);
   }
   return 0;
 }
