@@ -3,7 +3,7 @@
 // carried state, sm_100a.  ABI: the EXTENSIONS of include/reax_abi.h.
 #include "delta_chunk.cuh"
 #include "kvcache.cuh"
-#include "paged.cuh"
+#include "paged_launch.cuh"
 
 REAX_DEFINE_STATUS_EXPORT()
 REAX_DEFINE_KV_EXPORTS()

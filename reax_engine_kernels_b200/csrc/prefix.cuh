@@ -1,0 +1,343 @@
+// Attention of a whole batch over the prefix that its sequences share (reax_fmha_paged with a prefix), sm_100a tcgen05.
+//
+// The B * M query rows of a key/value head are one matrix: with 64 sequences of 4 rows each it is 256 rows against the same
+// keys, and the prefix is read (and dequantised) once per 128 rows instead of once per sequence.  The result is a partial output
+// and the log2 of its sum for each row and chunk of the prefix, as paged_kernel leaves them; paged_join_kernel joins all.
+//
+// One CTA per SM takes 128 rows of one head and a chunk of the keys, 64 at a time.  13 warps:
+//   0..3    softmax, a thread per row (TMEM lane): S out of TMEM, P (f16) back over it;
+//   4..11   loads and dequantisation: 16 cache bytes -> 16 f16 -> 128-byte-swizzled shared memory, each warp eight rows of K and of
+//           V per tile, the next tile's bytes in registers while the current one waits for its buffer;
+//   12      one thread issues S_j = Q K_j^T (M = 128, N = 64, K = D), then O += P_{j-1} V_{j-1} (N = D, K = 64, P from TMEM).
+// K and V have two buffers each, S two, freed by tcgen05.commit.  The products of a tile take about 1100 cycles of the tensor pipe at
+// D = 256, the conversions about 400 of the ALU's, the exponents 512 of the MUFU's.
+//
+// The rows' powers of two go into the f16 values, relative to the tile's largest (nk, nv): e4m3 has 4 bits, f16 11, and a row stays
+// exact down to 2^-12 of the tile's largest row, and right to 2^-12 of its own largest value down to 2^-20.  What is
+// left is one factor per tile, so a score costs one multiply-add and one exponent: P = 2^(x - m + nv - ref + 12), ref the
+// running maximum of the tiles' nv, m a lazy maximum that no x passes by more than 2 (P < 2^15).  The 12 keeps f16's
+// full precision down to 2^-26.  (Both powers of two applied to the scores, as paged_kernel does it, made the softmax the
+// bound: 254 us for 64 questions on a shared document of 32768 tokens.)  O and the sum carry 2^-ref and 2^12 until the end.
+// A row whose K or V is NaN becomes a NaN key and a zero value, which reaches the queries that see it and no others.
+#pragma once
+#include "paged.cuh"
+
+namespace reax {
+
+constexpr int PF_BN = 64, PF_ROWS = 128, PF_THREADS = 13 * 32;
+
+template <int D>
+struct PrefixCfg {
+  static constexpr uint32_t Q_BYTES = PF_ROWS * D * 2, KV_BYTES = PF_BN * D * 2;
+  static constexpr uint32_t O_COL = 128, TMEM_COLS = D == 256 ? 512 : 256;  // S (then P) at columns 0 and 64, O from 128 on
+  static constexpr int SMEM = 1024 + Q_BYTES + 4 * KV_BYTES;
+};
+
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N, int b_mn_major = 0) {
+  return idesc_bf16(M, N, b_mn_major) & ~((1u << 7) | (1u << 10));  // format 0 of A and B: f16
+}
+
+// grid (tiles of 128 rows * chunks of the prefix, H)
+template <int D>
+__global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_constant__ PagedArgs a) {
+  using C = PrefixCfg<D>;
+  extern __shared__ uint8_t pf_raw[];
+  __shared__ __align__(8) uint64_t bars[16];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  __shared__ float srow[PF_ROWS];
+  __shared__ int skn[2], svn[2];            // a tile's largest nk and nv
+  __shared__ unsigned long long slive[2];  // its keys that exist
+  pdl_launch();  // the own keys' kernel needs nothing from here
+  const uint32_t base = (smem_u32(pf_raw) + 1023u) & ~1023u;
+  const uint32_t sq = base, sk = sq + C::Q_BYTES, sv = sk + 2 * C::KV_BYTES;
+  const int split = blockIdx.x % a.psplits, R0 = blockIdx.x / a.psplits * PF_ROWS, h = blockIdx.y;
+  const int lane = threadIdx.x & 31, warp = warp_id();
+  const int c0 = split * a.pchunk, c1 = min(a.Lp, c0 + a.pchunk), ntiles = (c1 - c0 + PF_BN - 1) / PF_BN;
+  const int rows = a.B * a.M;
+  auto bar = [&](int i) { return smem_u32(&bars[i]); };
+  // kfull 0,1  vfull 2,3  kempty 4,5  vempty 6,7  s_ready 8,9  p_ready 10,11  pv_done 12,13  drain 14
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 4; ++i) mbar_init(bar(i), 8);
+    for (int i = 4; i < 10; ++i) mbar_init(bar(i), 1);
+    mbar_init(bar(10), 4);
+    mbar_init(bar(11), 4);
+    for (int i = 12; i < 15; ++i) mbar_init(bar(i), 1);
+    abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 12) {
+    tmem_alloc(smem_u32(&tmem_slot), C::TMEM_COLS);
+    tmem_relinquish();
+  } else {  // q: each row scaled by its power of two (and by the scale's sign), f16, swizzled
+    constexpr int LPR = D / 8, RPW = 32 / LPR;  // lanes per row, rows per warp and pass
+    const int sub = lane % LPR;
+    for (int r = warp * RPW + lane / LPR; r < PF_ROWS; r += 12 * RPW) {
+      const int R = R0 + r, b = R / a.M, m = R % a.M;
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (R < rows) x = *reinterpret_cast<const uint4*>(a.q + b * a.qB + h * a.qH + m * a.qM + sub * 8);
+      uint32_t top = max_u16x2(max_u16x2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), max_u16x2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
+      top = max(top & 0xffffu, top >> 16);
+      const uint32_t lanes = LPR == 32 ? 0xffffffffu : 0xffffu << (lane & 16);
+#pragma unroll
+      for (int o = LPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(lanes, top, o));
+      const int e = min(max((int)(top >> 7), 2), 252);
+      const float inv = __uint_as_float((uint32_t)(254 - e) << 23) * (a.scale_log2 < 0.f ? -1.f : 1.f);
+      if (sub == 0) srow[r] = __uint_as_float((uint32_t)e << 23) * fabsf(a.scale_log2);
+      st_shared_v4(sq + (sub >> 3) * (PF_ROWS * 128) + r * 128 + (((sub & 7) ^ (r & 7)) << 4),
+                   make_uint4(pack_f16(bf_lo(x.x) * inv, bf_hi(x.x) * inv), pack_f16(bf_lo(x.y) * inv, bf_hi(x.y) * inv),
+                              pack_f16(bf_lo(x.z) * inv, bf_hi(x.z) * inv), pack_f16(bf_lo(x.w) * inv, bf_hi(x.w) * inv)));
+    }
+    fence_proxy_async_smem();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  volatile int* abort = &abort_flag;
+
+  if (warp >= 4 && warp < 12) {  // ---------------------------------------------------------------- dequantisation
+    const int w = warp - 4, r8 = lane & 7, cq = lane >> 3, row = w * 8 + r8;
+    constexpr int U = D / 64;  // 16-byte units of a row per lane
+    const uint8_t *kb = a.kc + h * a.cH, *vb = a.vc + h * a.cH;
+    uint4 kx[U], vx[U];
+    uint32_t kbytes = 0, vbytes = 0;  // exponent bytes of keys 2 lane, 2 lane + 1 of the tile
+    bool ok2 = false, odd_ok = false;
+    auto page_of = [&](int key, int& off, bool& ok) {
+      const int pi = a.shift >= 0 ? key >> a.shift : key / a.page;
+      off = key - pi * a.page;
+      const long long pid = key < c1 ? a.prefix[pi] : -1;
+      ok = pid >= 0 && pid < a.pages;
+      if (key < c1 && !ok) record_status(ST_BAD_PAGE);
+      return ok ? pid : 0;
+    };
+    auto load = [&](int j) {
+      const int k0 = c0 + j * PF_BN;
+      int off;
+      bool ok;
+      long long pid = page_of(k0 + w * 8, off, ok);  // eight rows lie in one page
+      ok = ok && k0 + row < c1;
+      const long long at = pid * a.cP + (long long)(off + r8) * D + cq * 16;
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        kx[i] = ok ? __ldg(reinterpret_cast<const uint4*>(kb + at + i * 64)) : make_uint4(0, 0, 0, 0);
+        vx[i] = ok ? __ldg(reinterpret_cast<const uint4*>(vb + at + i * 64)) : make_uint4(0, 0, 0, 0);
+      }
+      pid = page_of(k0 + 2 * lane, off, ok2);  // every warp reads all 64 keys' exponents
+      odd_ok = ok2 && k0 + 2 * lane + 1 < c1;
+      const long long es = pid * a.eP + h * a.eH + off;
+      kbytes = ok2 ? *reinterpret_cast<const uint16_t*>(a.ke + es) : 0u;
+      vbytes = ok2 ? *reinterpret_cast<const uint16_t*>(a.ve + es) : 0u;
+    };
+    auto put = [&](uint32_t buf, const uint4 (&x)[U], uint32_t scale, uint32_t fill) {
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const uint32_t y[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+        const int c = 2 * (i * 4 + cq);  // first of two 16-byte chunks of the f16 row
+        const uint32_t dst = buf + (c >> 3) * (PF_BN * 128) + row * 128;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          uint32_t z[4];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const uint32_t v = e4m3x2_f16x2((uint16_t)(n & 1 ? y[2 * k + (n >> 1)] >> 16 : y[2 * k + (n >> 1)]));
+            asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(z[n]) : "r"(v), "r"(scale), "r"(fill));
+          }
+          st_shared_v4(dst + ((((c & 7) + k) ^ r8) << 4), make_uint4(z[0], z[1], z[2], z[3]));
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+    };
+    // f16x2 of 2^(n - top), 0 below f16's range
+    auto scale_of = [&](int n, int top) {
+      const int e = n - top;
+      const uint32_t b = e >= -14 ? (uint32_t)(e + 15) << 10 : e >= -24 ? 1u << (e + 24) : 0u;
+      return b | (b << 16);
+    };
+    load(0);
+    for (int j = 0; j < ntiles; ++j) {
+      const int s = j & 1;
+      const uint32_t par = ((j >> 1) & 1) ^ 1;  // the buffer's previous use, done; the first two pass at once
+      // exponents: NaN rows and keys that do not exist take no part in the maxima
+      const int k2[2] = {(int)(kbytes & 255u), (int)(kbytes >> 8)}, v2[2] = {(int)(vbytes & 255u), (int)(vbytes >> 8)};
+      int kn = 0, vn = 0;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if ((e ? odd_ok : ok2) && k2[e] != 255 && v2[e] != 255) kn = max(kn, k2[e]), vn = max(vn, v2[e]);
+      kn = __reduce_max_sync(0xffffffffu, kn);
+      vn = __reduce_max_sync(0xffffffffu, vn);
+      const uint32_t even = __ballot_sync(0xffffffffu, ok2), odd = __ballot_sync(0xffffffffu, odd_ok);
+      const int src = row >> 1;
+      const uint32_t kp = __shfl_sync(0xffffffffu, kbytes, src), vp = __shfl_sync(0xffffffffu, vbytes, src);
+      const int nk = row & 1 ? kp >> 8 : kp & 255u, nv = row & 1 ? vp >> 8 : vp & 255u;
+      const bool nan = nk == 255 || nv == 255;
+      if (!mbar_wait_warp(bar(4 + s), par, abort, ST_TIMEOUT_ATTN)) break;
+      put(sk + s * C::KV_BYTES, kx, nan ? 0u : scale_of(nk, kn), nan ? 0x7e007e00u : 0u);
+      if (lane == 0) mbar_arrive(bar(s));
+      if (!mbar_wait_warp(bar(6 + s), par, abort, ST_TIMEOUT_ATTN)) break;
+      put(sv + s * C::KV_BYTES, vx, nan ? 0u : scale_of(nv, vn), 0u);
+      if (w == 0 && lane == 0) {
+        skn[s] = kn - 127;
+        svn[s] = vn - 127;
+        unsigned long long live = 0;
+        for (int i = 0; i < 32; ++i) live |= (unsigned long long)(((even >> i) & 1u) | (((odd >> i) & 1u) << 1)) << (2 * i);
+        slive[s] = live;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(2 + s));
+      if (j + 1 < ntiles) load(j + 1);
+    }
+  } else if (warp == 12) {  // --------------------------------------------------------------------- MMA issue
+    if (lane == 0) {
+      constexpr uint32_t IDESC_S = idesc_f16(PF_ROWS, PF_BN), IDESC_PV = idesc_f16(PF_ROWS, D, /*b_mn_major=*/1);
+      bool live = true;
+      for (int j = 0; j <= ntiles && live; ++j) {
+        if (j < ntiles) {
+          const int s = j & 1;
+          live = mbar_wait(bar(s), (j >> 1) & 1, abort, ST_TIMEOUT_ATTN);
+          if (!live) break;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            mma_bf16_ss(tmem + s * 64, sw128_desc(sq + (kk >> 2) * (PF_ROWS * 128) + (kk & 3) * 32),
+                        sw128_desc(sk + s * C::KV_BYTES + (kk >> 2) * (PF_BN * 128) + (kk & 3) * 32), IDESC_S, kk > 0);
+          mma_commit(bar(4 + s));
+          mma_commit(bar(8 + s));
+        }
+        if (j > 0) {
+          const int i = j - 1, s = i & 1;
+          live = mbar_wait(bar(10 + s), (i >> 1) & 1, abort, ST_TIMEOUT_ATTN) &&
+                 mbar_wait(bar(2 + s), (i >> 1) & 1, abort, ST_TIMEOUT_ATTN);
+          if (!live) break;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < PF_BN / 16; ++kk)
+            mma_bf16_ts(tmem + C::O_COL, tmem + s * 64 + kk * 8,
+                        sw128_desc(sv + s * C::KV_BYTES + kk * 2048, /*lbo=*/PF_BN * 128, /*sbo=*/1024), IDESC_PV, i > 0 || kk > 0);
+          mma_commit(bar(6 + s));
+          mma_commit(bar(12 + s));
+        }
+      }
+      // whatever was issued ends before the CTA gives its memory back
+      mma_commit(bar(14));
+      const long long t0 = clock64();
+      while (!mbar_try_wait(bar(14), 0))
+        if (clock64() - t0 > REAX_DRAIN_LIMIT) {
+          record_status(ST_TIMEOUT_DRAIN);
+          break;
+        }
+    }
+    __syncwarp();
+  } else if (warp < 4) {  // ----------------------------------------------------------------------- softmax
+    const int row = warp * 32 + lane, R = R0 + row;
+    const bool real = R < rows;
+    const int b = real ? R / a.M : 0, mr = real ? R % a.M : 0;
+    const int lim = real ? min(a.qpos[b * a.qpB + mr / a.G], a.Lp - 1) : a.Lp - 1;
+    const float rs = srow[row];
+    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+    float m = -INFINITY, l = 0.f;
+    int ref = -127;
+    bool live = true;
+    for (int j = 0; j < ntiles; ++j) {
+      const int s = j & 1;
+      live = mbar_wait_warp(bar(8 + s), (j >> 1) & 1, abort, ST_TIMEOUT_ATTN) &&
+             mbar_wait_warp(bar(2 + s), (j >> 1) & 1, abort, ST_TIMEOUT_ATTN);  // the tile's exponents come with V
+      if (!live) break;
+      tc_fence_after();
+      uint32_t x[64];
+      tmem_ld64(lanes + s * 64, x);
+      const int k0 = c0 + j * PF_BN, vn = svn[s];
+      const unsigned long long have = slive[s];
+      float c1s = rs * pow2_byte((uint32_t)(skn[s] + 127));
+      if (c1s < 0x1p-126f) c1s = 0x1p-126f;  // not 0: a masked score is -inf
+      if (__any_sync(0xffffffffu, k0 + PF_BN - 1 > lim || have != ~0ull)) {
+#pragma unroll
+        for (int i = 0; i < 64; ++i)
+          if (k0 + i > lim || !((have >> i) & 1ull)) x[i] = 0xff800000u;  // -inf
+      }
+      float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 64; i += 4) {
+        t0 = max3f(t0, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+        t1 = max3f(t1, __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
+      }
+      t0 = fmaxf(t0, t1);
+      const float mx = t0 == -INFINITY ? t0 : t0 * c1s;
+      if (__any_sync(0xffffffffu, mx > m + 2.f) || vn > ref) {  // raise the references, rescale what there is
+        const float mn = fmaxf(mx, m);
+        const int rn = max(vn, ref);
+        const float al = ex2_approx(m - finite_or_zero(mn));
+        l *= al;
+        m = mn;
+        if (j > 0) {
+          const float ao = al * ex2_approx((float)(ref - rn));
+          live = mbar_wait_warp(bar(12 + (s ^ 1)), ((j - 1) >> 1) & 1, abort, ST_TIMEOUT_ATTN);
+          if (!live) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(lanes + C::O_COL + c, o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * ao);
+            tmem_st32_nowait(lanes + C::O_COL + c, o);
+          }
+          tmem_wait_st();
+        }
+        ref = rn;
+      }
+      // at = nv - ref: a tile of values 2^100 smaller than another's adds nothing, but its weights still count in the sum
+      const float at = (float)max(vn - ref, -100), c0s = at + 12.f - finite_or_zero(m);
+      float sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float p0 = ex2_approx(__fmaf_rn(__uint_as_float(x[c * 16 + 2 * i]), c1s, c0s));
+          const float p1 = ex2_approx(__fmaf_rn(__uint_as_float(x[c * 16 + 2 * i + 1]), c1s, c0s));
+          sum += p0 + p1;
+          y[i] = pack_f16(p0, p1);
+        }
+        tmem_st8_nowait(lanes + s * 64 + c * 8, y);
+      }
+      l = __fmaf_rn(sum, ex2_approx(-at - 12.f), l);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(10 + s));
+    }
+    if (live) live = mbar_wait_warp(bar(12 + ((ntiles - 1) & 1)), ((ntiles - 1) >> 1) & 1, abort, ST_TIMEOUT_ATTN);
+    const long long out = (long long)(a.splits + split) * a.B * a.H * a.M + ((long long)b * a.H + h) * a.M + mr;
+    if (live) {
+      tc_fence_after();
+      const float fac = l == 0.f ? 0.f : pow2_byte((uint32_t)(ref + 127)) * 0x1p-12f / l;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        uint32_t o[32];
+        tmem_ld32(lanes + C::O_COL + c, o);
+        if (real) {
+          float4* p = reinterpret_cast<float4*>(a.part + out * D + c);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = l == 0.f ? 0.f : __uint_as_float(o[4 * e + k]) * fac;
+            p[e] = make_float4(v[0], v[1], v[2], v[3]);
+          }
+        }
+      }
+    }
+    // after a wait that ran out the rows are NaN, not what the workspace held
+    if (real) a.lse[out] = !live ? __uint_as_float(0x7fc00000u) : l == 0.f ? -INFINITY : m + log2f(l);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::TMEM_COLS);
+  }
+}
+
+}  // namespace reax

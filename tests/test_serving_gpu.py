@@ -285,11 +285,13 @@ def test_rows_that_see_part_of_the_prefix_or_nothing(D):
     assert rk.fmha_paged(q, c, none, 0.07, qpos=qpos, G=2).count_nonzero() == 0
 
 
-@pytest.mark.parametrize("Lp", [0, 130])
-def test_masked_rows_may_hold_anything(Lp):
+# G = 4 rows a sequence keep the prefix with the kernel for few rows, more take it to the one of 128-row tiles
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("G,Lp", [(4, 0), (4, 130), (8, 130), (50, 130)])
+def test_masked_rows_may_hold_anything(G, Lp, D):
     """Bytes behind a sequence's end: NaN codes and NaN exponents, in its last page and in the prefix's."""
     lens = [5, 70, 16]
-    q, c, table, qpos, prefix = setup(11, 3, 2, 4, 1, 128, 32, lens, Lp)
+    q, c, table, qpos, prefix = setup(11, 3, 2, G, 1, D, 32, lens, Lp)
     for t in (c.k, c.v):
         u = t.view(torch.uint8)
         for b, n in enumerate(lens):
@@ -303,46 +305,60 @@ def test_masked_rows_may_hold_anything(Lp):
                 t[table[b, n // 32].long(), :, n % 32:] = 255
         if Lp:
             t[prefix[-1].long(), :, Lp % 32:] = 255
-    o = rk.fmha_paged(q, c, table, 0.1, qpos=qpos, G=4, prefix=prefix if Lp else None, prefix_len=Lp)
+    o = rk.fmha_paged(q, c, table, 0.1, qpos=qpos, G=G, prefix=prefix if Lp else None, prefix_len=Lp)
     assert torch.isfinite(o).all()
-    assert_attention(o, q, c, table, 0.1, qpos, 4, prefix if Lp else None, Lp)
+    assert_attention(o, q, c, table, 0.1, qpos, G, prefix if Lp else None, Lp)
 
 
-@pytest.mark.parametrize("Lp", [0, 100])
-def test_nan_rows_reach_only_the_queries_that_see_them(Lp):
+@pytest.mark.parametrize("G,Lp", [(2, 0), (2, 100), (4, 100)])
+def test_nan_rows_reach_only_the_queries_that_see_them(G, Lp):
     """A NaN key (or value) row among a sequence's new tokens: queries before it are finite, the others NaN."""
-    q, c, table, qpos, prefix = setup(12, 2, 1, 2, 4, 128, 16, [40, 41], Lp)
+    q, c, table, qpos, prefix = setup(12, 2, 1, G, 4, 128, 16, [40, 41], Lp)
     p, off = table[0, 38 // 16].long(), 38 % 16
     c.ke[p, 0, off] = 255
     p, off = table[1, 40 // 16].long(), 40 % 16
     c.ve[p, 0, off] = 255
-    o = rk.fmha_paged(q, c, table, 0.1, qpos=qpos, G=2, prefix=prefix if Lp else None, prefix_len=Lp)
-    assert_attention(o, q, c, table, 0.1, qpos, 2, prefix if Lp else None, Lp)
+    o = rk.fmha_paged(q, c, table, 0.1, qpos=qpos, G=G, prefix=prefix if Lp else None, prefix_len=Lp)
+    assert_attention(o, q, c, table, 0.1, qpos, G, prefix if Lp else None, Lp)
 
 
-def test_far_magnitudes():
+@pytest.mark.parametrize("G", [2, 4])
+@pytest.mark.parametrize("D", [128, 256])
+def test_nan_rows_in_the_prefix(G, D):
+    """A NaN key row, and a NaN value row, of the prefix: only rows whose qpos lies before them are finite."""
+    for which in ("ke", "ve"):
+        q, c, table, qpos, prefix = setup(33, 2, 1, G, 4, D, 16, [40, 41], 150)
+        getattr(c, which)[prefix[99 // 16].long(), 0, 99 % 16] = 255
+        qpos[0] = torch.tensor([20, 98, 99, 149], dtype=torch.int32)
+        o = rk.fmha_paged(q, c, table, 0.1, qpos=qpos, G=G, prefix=prefix, prefix_len=150)
+        assert torch.isfinite(o[0, :, :2 * G]).all() and torch.isnan(o[0, :, 2 * G:]).all() and torch.isnan(o[1]).all()
+        assert_attention(o, q, c, table, 0.1, qpos, G, prefix, 150)
+
+
+@pytest.mark.parametrize("G", [3, 8])
+def test_far_magnitudes(G):
     """Queries and rows of very different powers of two, a scale below zero, an outlier channel."""
     for D, scale, spread in ((128, 0.1, 4.0), (256, -0.05, 2.0), (128, 1e-3, 8.0)):
-        q, c, table, qpos, prefix = setup(13 + D, 3, 2, 3, 1, D, 16, [50, 200, 333], 90, spread)
+        q, c, table, qpos, prefix = setup(13 + D, 3, 2, G, 1, D, 16, [50, 200, 333], 90, spread)
         q[0] *= 1e-20
         q[1, :, :, 5] *= 300
         q[2] *= 2.0 ** 20
         sc = scale if spread < 8 else scale * 1e-3
         q[2] *= 2.0 ** -18
-        o = rk.fmha_paged(q, c, table, sc, qpos=qpos, G=3, prefix=prefix, prefix_len=90)
-        assert_attention(o, q, c, table, sc, qpos, 3, prefix, 90)
+        o = rk.fmha_paged(q, c, table, sc, qpos=qpos, G=G, prefix=prefix, prefix_len=90)
+        assert_attention(o, q, c, table, sc, qpos, G, prefix, 90)
 
 
-@pytest.mark.parametrize("Lp", [0, 64])
-def test_page_ids_out_of_range_are_not_seen_and_reported(Lp):
-    q, c, table, qpos, prefix = setup(14, 2, 2, 2, 1, 128, 32, [100, 90], Lp)
+@pytest.mark.parametrize("G,Lp", [(2, 0), (2, 64), (20, 64)])
+def test_page_ids_out_of_range_are_not_seen_and_reported(G, Lp):
+    q, c, table, qpos, prefix = setup(14, 2, 2, G, 1, 128, 32, [100, 90], Lp)
     n = c.k.shape[0]
     table[0, 1], table[1, 0] = n, -1
     if Lp:
         prefix[1] = 1 << 30
-    o = rk.fmha_paged(q, c, table, 0.1, qpos=qpos, G=2, prefix=prefix if Lp else None, prefix_len=Lp)
+    o = rk.fmha_paged(q, c, table, 0.1, qpos=qpos, G=G, prefix=prefix if Lp else None, prefix_len=Lp)
     assert status() == 0x502
-    assert_attention(o, q, c, table, 0.1, qpos, 2, prefix if Lp else None, Lp, bad=(n, -1, 1 << 30))
+    assert_attention(o, q, c, table, 0.1, qpos, G, prefix if Lp else None, Lp, bad=(n, -1, 1 << 30))
 
 
 def test_strided_operands():
