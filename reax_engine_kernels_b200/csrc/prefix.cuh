@@ -8,16 +8,18 @@
 //   0..3    softmax, a thread per row (TMEM lane): S out of TMEM, P (f16) back over it;
 //   4..11   loads and dequantisation: 16 cache bytes -> 16 f16 -> 128-byte-swizzled shared memory, each warp eight rows of K and of
 //           V per tile, the next tile's bytes in registers while the current one waits for its buffer;
-//   12      one thread issues S_j = Q K_j^T (M = 128, N = 64, K = D), then O += P_{j-1} V_{j-1} (N = D, K = 64, P from TMEM).
+//   12      one thread issues S_j = Q K_j^T (M = 128, N = 64, K = D), then O += P_{j-1} V_{j-1} (N = D, K = 64).
 // K and V have two buffers each, S two, freed by tcgen05.commit.  The products of a tile take about 1100 cycles of the tensor pipe at
-// D = 256, the conversions about 400 of the ALU's, the exponents 512 of the MUFU's.
+// D = 256, the conversions about 400 of the ALU's, the exponents 512 of the MUFU's; what they share is the shared-memory
+// port, where the f16 rows are written and read once (1024 cycles) and the cache's bytes pass.  So q and P are operands out of
+// tensor memory (q out of shared memory would be another 512 cycles a tile).
 //
 // The rows' powers of two go into the f16 values, relative to the tile's largest (nk, nv): e4m3 has 4 bits, f16 11, and a row stays
 // exact down to 2^-12 of the tile's largest row, and right to 2^-12 of its own largest value down to 2^-20.  What is
-// left is one factor per tile, so a score costs one multiply-add and one exponent: P = 2^(x - m + nv - ref + 12), ref the
-// running maximum of the tiles' nv, m a lazy maximum that no x passes by more than 2 (P < 2^15).  The 12 keeps f16's
-// full precision down to 2^-26.  (Both powers of two applied to the scores, as paged_kernel does it, made the softmax the
-// bound: 254 us for 64 questions on a shared document of 32768 tokens.)  O and the sum carry 2^-ref and 2^12 until the end.
+// left is one factor per tile, so a score costs one multiply-add and one exponent: P = 2^(x - m + nv - ref + 7), ref the
+// running maximum of the tiles' nv, m a lazy maximum that no x passes by more than 8 (P < 2^15).  The 7 keeps f16's
+// full precision down to 2^-21.  (Raising m costs a pass over O in tensor memory: with 2 in place of the 8 most tiles did.)  (Both powers of two applied to the scores, as paged_kernel does it, made the softmax the
+// bound: 254 us for 64 questions on a shared document of 32768 tokens.)  O carries 2^-ref and 2^7 until the end.
 // A row whose K or V is NaN becomes a NaN key and a zero value, which reaches the queries that see it and no others.
 #pragma once
 #include "paged.cuh"
@@ -28,13 +30,30 @@ constexpr int PF_BN = 64, PF_ROWS = 128, PF_THREADS = 13 * 32;
 
 template <int D>
 struct PrefixCfg {
-  static constexpr uint32_t Q_BYTES = PF_ROWS * D * 2, KV_BYTES = PF_BN * D * 2;
-  static constexpr uint32_t O_COL = 128, TMEM_COLS = D == 256 ? 512 : 256;  // S (then P) at columns 0 and 64, O from 128 on
-  static constexpr int SMEM = 1024 + Q_BYTES + 4 * KV_BYTES;
+  static constexpr uint32_t KV_BYTES = PF_BN * D * 2;
+  static constexpr uint32_t Q_COL = 128, O_COL = 256, TMEM_COLS = 512;  // S (then P) at columns 0 and 64
+  static constexpr int SMEM = 1024 + 4 * KV_BYTES;
 };
 
 __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, int b_mn_major = 0) {
   return idesc_bf16(M, N, b_mn_major) & ~((1u << 7) | (1u << 10));  // format 0 of A and B: f16
+}
+
+// Loads that are to be issued where they stand: the compiler moves a plain read-only load down to its use, here a tile later.
+__device__ __forceinline__ uint4 ld_early_v4(const void* p) {
+  uint4 x;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "l"(p));
+  return x;
+}
+__device__ __forceinline__ uint32_t ld_early_u16(const void* p) {
+  uint16_t x;
+  asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(x) : "l"(p));
+  return x;
+}
+__device__ __forceinline__ int ld_early_s32(const int* p) {
+  int x;
+  asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(x) : "l"(p));
+  return x;
 }
 
 // grid (tiles of 128 rows * chunks of the prefix, H)
@@ -45,50 +64,30 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
   __shared__ __align__(8) uint64_t bars[16];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
-  __shared__ float srow[PF_ROWS];
   __shared__ int skn[2], svn[2];            // a tile's largest nk and nv
-  __shared__ unsigned long long slive[2];  // its keys that exist
+  __shared__ uint32_t seven[2], sodd[2];    // its even and odd keys that exist
   pdl_launch();  // the own keys' kernel needs nothing from here
   const uint32_t base = (smem_u32(pf_raw) + 1023u) & ~1023u;
-  const uint32_t sq = base, sk = sq + C::Q_BYTES, sv = sk + 2 * C::KV_BYTES;
+  const uint32_t sk = base, sv = sk + 2 * C::KV_BYTES;
   const int split = blockIdx.x % a.psplits, R0 = blockIdx.x / a.psplits * PF_ROWS, h = blockIdx.y;
   const int lane = threadIdx.x & 31, warp = warp_id();
   const int c0 = split * a.pchunk, c1 = min(a.Lp, c0 + a.pchunk), ntiles = (c1 - c0 + PF_BN - 1) / PF_BN;
   const int rows = a.B * a.M;
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
-  // kfull 0,1  vfull 2,3  kempty 4,5  vempty 6,7  s_ready 8,9  p_ready 10,11  pv_done 12,13  drain 14
+  // kfull 0,1  vfull 2,3  kempty 4,5  vempty 6,7  s_ready 8,9  p_ready 10,11  pv_done 12,13  drain 14  q_ready 15
   if (threadIdx.x == 0) {
     for (int i = 0; i < 4; ++i) mbar_init(bar(i), 8);
     for (int i = 4; i < 10; ++i) mbar_init(bar(i), 1);
     mbar_init(bar(10), 4);
     mbar_init(bar(11), 4);
     for (int i = 12; i < 15; ++i) mbar_init(bar(i), 1);
+    mbar_init(bar(15), 4);
     abort_flag = 0;
     fence_mbar_init();
   }
   if (warp == 12) {
     tmem_alloc(smem_u32(&tmem_slot), C::TMEM_COLS);
     tmem_relinquish();
-  } else {  // q: each row scaled by its power of two (and by the scale's sign), f16, swizzled
-    constexpr int LPR = D / 8, RPW = 32 / LPR;  // lanes per row, rows per warp and pass
-    const int sub = lane % LPR;
-    for (int r = warp * RPW + lane / LPR; r < PF_ROWS; r += 12 * RPW) {
-      const int R = R0 + r, b = R / a.M, m = R % a.M;
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (R < rows) x = *reinterpret_cast<const uint4*>(a.q + b * a.qB + h * a.qH + m * a.qM + sub * 8);
-      uint32_t top = max_u16x2(max_u16x2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), max_u16x2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
-      top = max(top & 0xffffu, top >> 16);
-      const uint32_t lanes = LPR == 32 ? 0xffffffffu : 0xffffu << (lane & 16);
-#pragma unroll
-      for (int o = LPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(lanes, top, o));
-      const int e = min(max((int)(top >> 7), 2), 252);
-      const float inv = __uint_as_float((uint32_t)(254 - e) << 23) * (a.scale_log2 < 0.f ? -1.f : 1.f);
-      if (sub == 0) srow[r] = __uint_as_float((uint32_t)e << 23) * fabsf(a.scale_log2);
-      st_shared_v4(sq + (sub >> 3) * (PF_ROWS * 128) + r * 128 + (((sub & 7) ^ (r & 7)) << 4),
-                   make_uint4(pack_f16(bf_lo(x.x) * inv, bf_hi(x.x) * inv), pack_f16(bf_lo(x.y) * inv, bf_hi(x.y) * inv),
-                              pack_f16(bf_lo(x.z) * inv, bf_hi(x.z) * inv), pack_f16(bf_lo(x.w) * inv, bf_hi(x.w) * inv)));
-    }
-    fence_proxy_async_smem();
   }
   tc_fence_before();
   __syncthreads();
@@ -97,53 +96,65 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
   volatile int* abort = &abort_flag;
 
   if (warp >= 4 && warp < 12) {  // ---------------------------------------------------------------- dequantisation
-    const int w = warp - 4, r8 = lane & 7, cq = lane >> 3, row = w * 8 + r8;
-    constexpr int U = D / 64;  // 16-byte units of a row per lane
+    // a load of a warp covers whole rows: LPR lanes a row, its unit i rows RPU i .. + RPU - 1 of the warp's eight
+    constexpr int LPR = D / 16, RPU = 32 / LPR, U = 8 / RPU;
+    const int w = warp - 4, r8 = lane & 7, row = w * 8 + r8, sub = lane % LPR, ur = lane / LPR;
+    const bool swap = (sub >> 2) & 1;  // which half goes first, so that eight lanes' stores fall in different banks
     const uint8_t *kb = a.kc + h * a.cH, *vb = a.vc + h * a.cH;
-    uint4 kx[U], vx[U];
-    uint32_t kbytes = 0, vbytes = 0;  // exponent bytes of keys 2 lane, 2 lane + 1 of the tile
-    bool ok2 = false, odd_ok = false;
-    auto page_of = [&](int key, int& off, bool& ok) {
+    struct Tile {  // what is loaded of a tile: 8 rows' bytes, and the exponent bytes of keys 2 lane, 2 lane + 1 of all 64
+      uint4 kx[U], vx[U];
+      uint32_t kbytes, vbytes;
+      bool even, odd;
+    };
+    int row_id = -1, row_off = 0, exp_id = -1, exp_off = 0;  // page and offset of the next tile to load: rows, exponents
+    auto page_of = [&](int key, int& off) {
       const int pi = a.shift >= 0 ? key >> a.shift : key / a.page;
       off = key - pi * a.page;
-      const long long pid = key < c1 ? a.prefix[pi] : -1;
-      ok = pid >= 0 && pid < a.pages;
-      if (key < c1 && !ok) record_status(ST_BAD_PAGE);
-      return ok ? pid : 0;
+      return key < c1 ? ld_early_s32(a.prefix + pi) : -1;
     };
-    auto load = [&](int j) {
+    auto pages = [&](int j) {
+      row_id = page_of(c0 + j * PF_BN + w * 8, row_off);  // eight rows lie in one page
+      exp_id = page_of(c0 + j * PF_BN + 2 * lane, exp_off);
+    };
+    // bytes of tile j; its page ids were loaded a tile ahead, as those of j + 1 are now
+    auto load = [&](int j, Tile& x) {
       const int k0 = c0 + j * PF_BN;
-      int off;
-      bool ok;
-      long long pid = page_of(k0 + w * 8, off, ok);  // eight rows lie in one page
-      ok = ok && k0 + row < c1;
-      const long long at = pid * a.cP + (long long)(off + r8) * D + cq * 16;
+      const long long rp = row_id, ep = exp_id;
+      const int ro = row_off, eo = exp_off;
+      if (j + 1 < ntiles) pages(j + 1);
+      const bool have = rp >= 0 && rp < a.pages;
+      const long long at = (have ? rp : 0) * a.cP + (long long)(ro + ur) * D + sub * 16;
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        kx[i] = ok ? __ldg(reinterpret_cast<const uint4*>(kb + at + i * 64)) : make_uint4(0, 0, 0, 0);
-        vx[i] = ok ? __ldg(reinterpret_cast<const uint4*>(vb + at + i * 64)) : make_uint4(0, 0, 0, 0);
+        const bool ok = have && k0 + w * 8 + i * RPU + ur < c1;
+        x.kx[i] = ok ? ld_early_v4(kb + at + i * RPU * D) : make_uint4(0, 0, 0, 0);
+        x.vx[i] = ok ? ld_early_v4(vb + at + i * RPU * D) : make_uint4(0, 0, 0, 0);
       }
-      pid = page_of(k0 + 2 * lane, off, ok2);  // every warp reads all 64 keys' exponents
-      odd_ok = ok2 && k0 + 2 * lane + 1 < c1;
-      const long long es = pid * a.eP + h * a.eH + off;
-      kbytes = ok2 ? *reinterpret_cast<const uint16_t*>(a.ke + es) : 0u;
-      vbytes = ok2 ? *reinterpret_cast<const uint16_t*>(a.ve + es) : 0u;
+      x.even = ep >= 0 && ep < a.pages;
+      x.odd = x.even && k0 + 2 * lane + 1 < c1;
+      if (!x.even && k0 + 2 * lane < c1) record_status(ST_BAD_PAGE);
+      const long long es = (x.even ? ep : 0) * a.eP + h * a.eH + eo;
+      x.kbytes = x.even ? ld_early_u16(a.ke + es) : 0u;
+      x.vbytes = x.even ? ld_early_u16(a.ve + es) : 0u;
     };
+    // scale: of row w * 8 + (lane & 7); all ones: a NaN row, filled with `fill`
     auto put = [&](uint32_t buf, const uint4 (&x)[U], uint32_t scale, uint32_t fill) {
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        const uint32_t y[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-        const int c = 2 * (i * 4 + cq);  // first of two 16-byte chunks of the f16 row
-        const uint32_t dst = buf + (c >> 3) * (PF_BN * 128) + row * 128;
+        const int r = i * RPU + ur, c = 2 * sub;  // first of two 16-byte chunks of the f16 row
+        const uint32_t sc = __shfl_sync(0xffffffffu, scale, r);
+        const uint32_t mul = sc == 0xffffffffu ? 0u : sc, add = sc == 0xffffffffu ? fill : 0u;
+        const uint32_t y[4] = {swap ? x[i].z : x[i].x, swap ? x[i].w : x[i].y, swap ? x[i].x : x[i].z, swap ? x[i].y : x[i].w};
+        const uint32_t dst = buf + (c >> 3) * (PF_BN * 128) + (w * 8 + r) * 128;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           uint32_t z[4];
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
             const uint32_t v = e4m3x2_f16x2((uint16_t)(n & 1 ? y[2 * k + (n >> 1)] >> 16 : y[2 * k + (n >> 1)]));
-            asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(z[n]) : "r"(v), "r"(scale), "r"(fill));
+            asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(z[n]) : "r"(v), "r"(mul), "r"(add));
           }
-          st_shared_v4(dst + ((((c & 7) + k) ^ r8) << 4), make_uint4(z[0], z[1], z[2], z[3]));
+          st_shared_v4(dst + (((((c & 7) + k) ^ (int)swap) ^ r) << 4), make_uint4(z[0], z[1], z[2], z[3]));
         }
       }
       fence_proxy_async_smem();
@@ -155,38 +166,47 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
       const uint32_t b = e >= -14 ? (uint32_t)(e + 15) << 10 : e >= -24 ? 1u << (e + 24) : 0u;
       return b | (b << 16);
     };
-    load(0);
-    for (int j = 0; j < ntiles; ++j) {
+    auto convert = [&](int j, const Tile& x) {
       const int s = j & 1;
       const uint32_t par = ((j >> 1) & 1) ^ 1;  // the buffer's previous use, done; the first two pass at once
       // exponents: NaN rows and keys that do not exist take no part in the maxima
-      const int k2[2] = {(int)(kbytes & 255u), (int)(kbytes >> 8)}, v2[2] = {(int)(vbytes & 255u), (int)(vbytes >> 8)};
+      const int k2[2] = {(int)(x.kbytes & 255u), (int)(x.kbytes >> 8)}, v2[2] = {(int)(x.vbytes & 255u), (int)(x.vbytes >> 8)};
       int kn = 0, vn = 0;
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        if ((e ? odd_ok : ok2) && k2[e] != 255 && v2[e] != 255) kn = max(kn, k2[e]), vn = max(vn, v2[e]);
+        if ((e ? x.odd : x.even) && k2[e] != 255 && v2[e] != 255) kn = max(kn, k2[e]), vn = max(vn, v2[e]);
       kn = __reduce_max_sync(0xffffffffu, kn);
       vn = __reduce_max_sync(0xffffffffu, vn);
-      const uint32_t even = __ballot_sync(0xffffffffu, ok2), odd = __ballot_sync(0xffffffffu, odd_ok);
-      const int src = row >> 1;
-      const uint32_t kp = __shfl_sync(0xffffffffu, kbytes, src), vp = __shfl_sync(0xffffffffu, vbytes, src);
+      const uint32_t even = __ballot_sync(0xffffffffu, x.even), odd = __ballot_sync(0xffffffffu, x.odd);
+      const uint32_t kp = __shfl_sync(0xffffffffu, x.kbytes, row >> 1), vp = __shfl_sync(0xffffffffu, x.vbytes, row >> 1);
       const int nk = row & 1 ? kp >> 8 : kp & 255u, nv = row & 1 ? vp >> 8 : vp & 255u;
       const bool nan = nk == 255 || nv == 255;
-      if (!mbar_wait_warp(bar(4 + s), par, abort, ST_TIMEOUT_ATTN)) break;
-      put(sk + s * C::KV_BYTES, kx, nan ? 0u : scale_of(nk, kn), nan ? 0x7e007e00u : 0u);
+      if (!mbar_wait_warp(bar(4 + s), par, abort, ST_TIMEOUT_ATTN)) return false;
+      put(sk + s * C::KV_BYTES, x.kx, nan ? 0xffffffffu : scale_of(nk, kn), 0x7e007e00u);
       if (lane == 0) mbar_arrive(bar(s));
-      if (!mbar_wait_warp(bar(6 + s), par, abort, ST_TIMEOUT_ATTN)) break;
-      put(sv + s * C::KV_BYTES, vx, nan ? 0u : scale_of(nv, vn), 0u);
+      if (!mbar_wait_warp(bar(6 + s), par, abort, ST_TIMEOUT_ATTN)) return false;
+      put(sv + s * C::KV_BYTES, x.vx, nan ? 0xffffffffu : scale_of(nv, vn), 0u);
       if (w == 0 && lane == 0) {
         skn[s] = kn - 127;
         svn[s] = vn - 127;
-        unsigned long long live = 0;
-        for (int i = 0; i < 32; ++i) live |= (unsigned long long)(((even >> i) & 1u) | (((odd >> i) & 1u) << 1)) << (2 * i);
-        slive[s] = live;
+        seven[s] = even;
+        sodd[s] = odd;
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(2 + s));
-      if (j + 1 < ntiles) load(j + 1);
+      return true;
+    };
+    // two tiles in registers: the next one's bytes arrive while this one is converted
+    Tile x0, x1;
+    pages(0);
+    load(0, x0);
+    for (int j = 0; j < ntiles; j += 2) {
+      if (j + 1 < ntiles) load(j + 1, x1);
+      if (!convert(j, x0)) break;
+      if (j + 1 < ntiles) {
+        if (j + 2 < ntiles) load(j + 2, x0);
+        if (!convert(j + 1, x1)) break;
+      }
     }
   } else if (warp == 12) {  // --------------------------------------------------------------------- MMA issue
     if (lane == 0) {
@@ -195,12 +215,12 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
       for (int j = 0; j <= ntiles && live; ++j) {
         if (j < ntiles) {
           const int s = j & 1;
-          live = mbar_wait(bar(s), (j >> 1) & 1, abort, ST_TIMEOUT_ATTN);
+          live = (j > 0 || mbar_wait(bar(15), 0, abort, ST_TIMEOUT_ATTN)) && mbar_wait(bar(s), (j >> 1) & 1, abort, ST_TIMEOUT_ATTN);
           if (!live) break;
           tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
-            mma_bf16_ss(tmem + s * 64, sw128_desc(sq + (kk >> 2) * (PF_ROWS * 128) + (kk & 3) * 32),
+            mma_bf16_ts(tmem + s * 64, tmem + C::Q_COL + kk * 8,
                         sw128_desc(sk + s * C::KV_BYTES + (kk >> 2) * (PF_BN * 128) + (kk & 3) * 32), IDESC_S, kk > 0);
           mma_commit(bar(4 + s));
           mma_commit(bar(8 + s));
@@ -234,8 +254,34 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
     const bool real = R < rows;
     const int b = real ? R / a.M : 0, mr = real ? R % a.M : 0;
     const int lim = real ? min(a.qpos[b * a.qpB + mr / a.G], a.Lp - 1) : a.Lp - 1;
-    const float rs = srow[row];
     const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+    // q: the row scaled by its power of two (and by the scale's sign), f16, into tensor memory
+    const uint16_t* qrow = a.q + b * a.qB + h * a.qH + mr * a.qM;
+    uint32_t top = 0;
+#pragma unroll 8
+    for (int c = 0; c < D / 8; ++c) {
+      const uint4 x = real ? *reinterpret_cast<const uint4*>(qrow + c * 8) : make_uint4(0, 0, 0, 0);
+      top = max_u16x2(top, max_u16x2(max_u16x2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), max_u16x2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
+    }
+    const int e = min(max((int)(max(top & 0xffffu, top >> 16) >> 7), 2), 252);
+    const float inv = __uint_as_float((uint32_t)(254 - e) << 23) * (a.scale_log2 < 0.f ? -1.f : 1.f);
+    const float rs = __uint_as_float((uint32_t)e << 23) * fabsf(a.scale_log2);
+#pragma unroll 4
+    for (int c = 0; c < D / 16; ++c) {
+      uint32_t y[8];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint4 x = real ? *reinterpret_cast<const uint4*>(qrow + c * 16 + k * 8) : make_uint4(0, 0, 0, 0);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[4 * k + i] = pack_f16(bf_lo(w[i]) * inv, bf_hi(w[i]) * inv);
+      }
+      tmem_st8_nowait(lanes + C::Q_COL + c * 8, y);
+    }
+    tmem_wait_st();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(15));
     float m = -INFINITY, l = 0.f;
     int ref = -127;
     bool live = true;
@@ -248,13 +294,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
       uint32_t x[64];
       tmem_ld64(lanes + s * 64, x);
       const int k0 = c0 + j * PF_BN, vn = svn[s];
-      const unsigned long long have = slive[s];
+      const uint32_t even = seven[s], odd = sodd[s];
       float c1s = rs * pow2_byte((uint32_t)(skn[s] + 127));
       if (c1s < 0x1p-126f) c1s = 0x1p-126f;  // not 0: a masked score is -inf
-      if (__any_sync(0xffffffffu, k0 + PF_BN - 1 > lim || have != ~0ull)) {
+      if (__any_sync(0xffffffffu, k0 + PF_BN - 1 > lim || (even & odd) != 0xffffffffu)) {
 #pragma unroll
         for (int i = 0; i < 64; ++i)
-          if (k0 + i > lim || !((have >> i) & 1ull)) x[i] = 0xff800000u;  // -inf
+          if (k0 + i > lim || !(((i & 1 ? odd : even) >> (i >> 1)) & 1u)) x[i] = 0xff800000u;  // -inf
       }
       float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
@@ -264,7 +310,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
       }
       t0 = fmaxf(t0, t1);
       const float mx = t0 == -INFINITY ? t0 : t0 * c1s;
-      if (__any_sync(0xffffffffu, mx > m + 2.f) || vn > ref) {  // raise the references, rescale what there is
+      if (__any_sync(0xffffffffu, mx > m + 8.f) || vn > ref) {  // raise the references, rescale what there is
         const float mn = fmaxf(mx, m);
         const int rn = max(vn, ref);
         const float al = ex2_approx(m - finite_or_zero(mn));
@@ -288,7 +334,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
         ref = rn;
       }
       // at = nv - ref: a tile of values 2^100 smaller than another's adds nothing, but its weights still count in the sum
-      const float at = (float)max(vn - ref, -100), c0s = at + 12.f - finite_or_zero(m);
+      const float at = (float)max(vn - ref, -100), c0s = at + 7.f - finite_or_zero(m);
       float sum = 0.f;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
@@ -302,7 +348,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
         }
         tmem_st8_nowait(lanes + s * 64 + c * 8, y);
       }
-      l = __fmaf_rn(sum, ex2_approx(-at - 12.f), l);
+      l = __fmaf_rn(sum, ex2_approx(-at - 7.f), l);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -312,7 +358,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
     const long long out = (long long)(a.splits + split) * a.B * a.H * a.M + ((long long)b * a.H + h) * a.M + mr;
     if (live) {
       tc_fence_after();
-      const float fac = l == 0.f ? 0.f : pow2_byte((uint32_t)(ref + 127)) * 0x1p-12f / l;
+      const float fac = l == 0.f ? 0.f : pow2_byte((uint32_t)(ref + 127)) * 0x1p-7f / l;
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         uint32_t o[32];
