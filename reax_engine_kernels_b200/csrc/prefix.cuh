@@ -4,10 +4,11 @@
 // keys, and the prefix is read (and dequantised) once per 128 rows instead of once per sequence.  The result is a partial output
 // and the log2 of its sum for each row and chunk of the prefix, as paged_kernel leaves them; paged_join_kernel joins all.
 //
-// One CTA per SM takes 128 rows of one head and a chunk of the keys, 64 at a time.  13 warps:
+// One CTA per SM takes 128 rows of one head and a chunk of the keys, 64 at a time.  14 warps:
 //   0..3    softmax, a thread per row (TMEM lane): S out of TMEM, P (f16) back over it;
-//   4..11   loads and dequantisation: 16 cache bytes -> 16 f16 -> 128-byte-swizzled shared memory, each warp eight rows of K and of
-//           V per tile, the next tile's bytes in registers while the current one waits for its buffer;
+//   4..11   dequantisation: 16 cache bytes -> 16 f16 in 128-byte-swizzled shared memory, each warp eight rows of K and of V per tile;
+//   13      bulk copies of the cache's bytes, 16 rows (always in one page) at a time, up to two (four) tiles ahead.  (Loads into
+//           registers by the dequantising warps took longer to issue than the conversion: 159 us for the shared document.)
 //   12      one thread issues S_j = Q K_j^T (M = 128, N = 64, K = D), then O += P_{j-1} V_{j-1} (N = D, K = 64).
 // K and V have two buffers each, S two, freed by tcgen05.commit.  The products of a tile take about 1100 cycles of the tensor pipe at
 // D = 256, the conversions about 400 of the ALU's, the exponents 512 of the MUFU's; what they share is the shared-memory
@@ -26,33 +27,31 @@
 
 namespace reax {
 
-constexpr int PF_BN = 64, PF_ROWS = 128, PF_THREADS = 13 * 32;
+constexpr int PF_BN = 64, PF_ROWS = 128, PF_THREADS = 14 * 32;
 
 template <int D>
 struct PrefixCfg {
   static constexpr uint32_t KV_BYTES = PF_BN * D * 2;
   static constexpr uint32_t Q_COL = 128, O_COL = 256, TMEM_COLS = 512;  // S (then P) at columns 0 and 64
-  static constexpr int SMEM = 1024 + 4 * KV_BYTES;
+  static constexpr int RAW = 2 * PF_BN * D, EXP = 2 * PF_BN;  // a tile as it lies in the cache: rows of K, of V; their exponents
+  static constexpr int NR = D == 256 ? 2 : 4;                 // tiles of it in flight
+  static constexpr int SMEM = 1024 + 4 * KV_BYTES + NR * (RAW + EXP);
 };
 
 __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, int b_mn_major = 0) {
   return idesc_bf16(M, N, b_mn_major) & ~((1u << 7) | (1u << 10));  // format 0 of A and B: f16
 }
 
-// Loads that are to be issued where they stand: the compiler moves a plain read-only load down to its use, here a tile later.
-__device__ __forceinline__ uint4 ld_early_v4(const void* p) {
-  uint4 x;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "l"(p));
-  return x;
+// bytes (a multiple of 16, both addresses 16-byte aligned) from global to shared memory; they count on the mbarrier
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
+               "r"(bar)
+               : "memory");
 }
-__device__ __forceinline__ uint32_t ld_early_u16(const void* p) {
+
+__device__ __forceinline__ uint32_t ld_shared_u16(uint32_t addr) {
   uint16_t x;
-  asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(x) : "l"(p));
-  return x;
-}
-__device__ __forceinline__ int ld_early_s32(const int* p) {
-  int x;
-  asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(x) : "l"(p));
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(addr) : "memory");
   return x;
 }
 
@@ -61,20 +60,22 @@ template <int D>
 __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_constant__ PagedArgs a) {
   using C = PrefixCfg<D>;
   extern __shared__ uint8_t pf_raw[];
-  __shared__ __align__(8) uint64_t bars[16];
+  __shared__ __align__(8) uint64_t bars[24];
+  __shared__ uint32_t sgran[4];  // which of a raw tile's four groups of 16 keys were copied
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   __shared__ int skn[2], svn[2];            // a tile's largest nk and nv
   __shared__ uint32_t seven[2], sodd[2];    // its even and odd keys that exist
   pdl_launch();  // the own keys' kernel needs nothing from here
   const uint32_t base = (smem_u32(pf_raw) + 1023u) & ~1023u;
-  const uint32_t sk = base, sv = sk + 2 * C::KV_BYTES;
+  const uint32_t sk = base, sv = sk + 2 * C::KV_BYTES, sraw = sv + 2 * C::KV_BYTES, sexp = sraw + C::NR * C::RAW;
   const int split = blockIdx.x % a.psplits, R0 = blockIdx.x / a.psplits * PF_ROWS, h = blockIdx.y;
   const int lane = threadIdx.x & 31, warp = warp_id();
   const int c0 = split * a.pchunk, c1 = min(a.Lp, c0 + a.pchunk), ntiles = (c1 - c0 + PF_BN - 1) / PF_BN;
   const int rows = a.B * a.M;
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
   // kfull 0,1  vfull 2,3  kempty 4,5  vempty 6,7  s_ready 8,9  p_ready 10,11  pv_done 12,13  drain 14  q_ready 15
+  // raw_full 16..19  raw_empty 20..23
   if (threadIdx.x == 0) {
     for (int i = 0; i < 4; ++i) mbar_init(bar(i), 8);
     for (int i = 4; i < 10; ++i) mbar_init(bar(i), 1);
@@ -82,6 +83,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
     mbar_init(bar(11), 4);
     for (int i = 12; i < 15; ++i) mbar_init(bar(i), 1);
     mbar_init(bar(15), 4);
+    for (int i = 0; i < 4; ++i) mbar_init(bar(16 + i), 1), mbar_init(bar(20 + i), 8);
     abort_flag = 0;
     fence_mbar_init();
   }
@@ -98,53 +100,21 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
   if (warp >= 4 && warp < 12) {  // ---------------------------------------------------------------- dequantisation
     // a load of a warp covers whole rows: LPR lanes a row, its unit i rows RPU i .. + RPU - 1 of the warp's eight
     constexpr int LPR = D / 16, RPU = 32 / LPR, U = 8 / RPU;
-    const int w = warp - 4, r8 = lane & 7, row = w * 8 + r8, sub = lane % LPR, ur = lane / LPR;
+    const int w = warp - 4, row = w * 8 + (lane & 7), sub = lane % LPR, ur = lane / LPR;
     const bool swap = (sub >> 2) & 1;  // which half goes first, so that eight lanes' stores fall in different banks
-    const uint8_t *kb = a.kc + h * a.cH, *vb = a.vc + h * a.cH;
-    struct Tile {  // what is loaded of a tile: 8 rows' bytes, and the exponent bytes of keys 2 lane, 2 lane + 1 of all 64
-      uint4 kx[U], vx[U];
-      uint32_t kbytes, vbytes;
-      bool even, odd;
-    };
-    int row_id = -1, row_off = 0, exp_id = -1, exp_off = 0;  // page and offset of the next tile to load: rows, exponents
-    auto page_of = [&](int key, int& off) {
-      const int pi = a.shift >= 0 ? key >> a.shift : key / a.page;
-      off = key - pi * a.page;
-      return key < c1 ? ld_early_s32(a.prefix + pi) : -1;
-    };
-    auto pages = [&](int j) {
-      row_id = page_of(c0 + j * PF_BN + w * 8, row_off);  // eight rows lie in one page
-      exp_id = page_of(c0 + j * PF_BN + 2 * lane, exp_off);
-    };
-    // bytes of tile j; its page ids were loaded a tile ahead, as those of j + 1 are now
-    auto load = [&](int j, Tile& x) {
-      const int k0 = c0 + j * PF_BN;
-      const long long rp = row_id, ep = exp_id;
-      const int ro = row_off, eo = exp_off;
-      if (j + 1 < ntiles) pages(j + 1);
-      const bool have = rp >= 0 && rp < a.pages;
-      const long long at = (have ? rp : 0) * a.cP + (long long)(ro + ur) * D + sub * 16;
+    // scale: of row w * 8 + (lane & 7); all ones: a row without values, filled with `fill`
+    auto put = [&](uint32_t buf, uint32_t raw, uint32_t scale, uint32_t fill) {
+      uint4 x[U];
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const bool ok = have && k0 + w * 8 + i * RPU + ur < c1;
-        x.kx[i] = ok ? ld_early_v4(kb + at + i * RPU * D) : make_uint4(0, 0, 0, 0);
-        x.vx[i] = ok ? ld_early_v4(vb + at + i * RPU * D) : make_uint4(0, 0, 0, 0);
-      }
-      x.even = ep >= 0 && ep < a.pages;
-      x.odd = x.even && k0 + 2 * lane + 1 < c1;
-      if (!x.even && k0 + 2 * lane < c1) record_status(ST_BAD_PAGE);
-      const long long es = (x.even ? ep : 0) * a.eP + h * a.eH + eo;
-      x.kbytes = x.even ? ld_early_u16(a.ke + es) : 0u;
-      x.vbytes = x.even ? ld_early_u16(a.ve + es) : 0u;
-    };
-    // scale: of row w * 8 + (lane & 7); all ones: a NaN row, filled with `fill`
-    auto put = [&](uint32_t buf, const uint4 (&x)[U], uint32_t scale, uint32_t fill) {
+      for (int i = 0; i < U; ++i) x[i] = ld_shared_v4(raw + (w * 8 + i * RPU) * D + lane * 16);
 #pragma unroll
       for (int i = 0; i < U; ++i) {
         const int r = i * RPU + ur, c = 2 * sub;  // first of two 16-byte chunks of the f16 row
         const uint32_t sc = __shfl_sync(0xffffffffu, scale, r);
-        const uint32_t mul = sc == 0xffffffffu ? 0u : sc, add = sc == 0xffffffffu ? fill : 0u;
-        const uint32_t y[4] = {swap ? x[i].z : x[i].x, swap ? x[i].w : x[i].y, swap ? x[i].x : x[i].z, swap ? x[i].y : x[i].w};
+        const bool none = sc == 0xffffffffu;
+        const uint32_t mul = none ? 0u : sc, add = none ? fill : 0u, keep = none ? 0u : 0xffffffffu;
+        const uint32_t y[4] = {(swap ? x[i].z : x[i].x) & keep, (swap ? x[i].w : x[i].y) & keep, (swap ? x[i].x : x[i].z) & keep,
+                               (swap ? x[i].y : x[i].w) & keep};
         const uint32_t dst = buf + (c >> 3) * (PF_BN * 128) + (w * 8 + r) * 128;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -166,26 +136,31 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
       const uint32_t b = e >= -14 ? (uint32_t)(e + 15) << 10 : e >= -24 ? 1u << (e + 24) : 0u;
       return b | (b << 16);
     };
-    auto convert = [&](int j, const Tile& x) {
-      const int s = j & 1;
+    for (int j = 0; j < ntiles; ++j) {
+      const int s = j & 1, rs = j % C::NR;
       const uint32_t par = ((j >> 1) & 1) ^ 1;  // the buffer's previous use, done; the first two pass at once
-      // exponents: NaN rows and keys that do not exist take no part in the maxima
-      const int k2[2] = {(int)(x.kbytes & 255u), (int)(x.kbytes >> 8)}, v2[2] = {(int)(x.vbytes & 255u), (int)(x.vbytes >> 8)};
+      const uint32_t raw = sraw + rs * C::RAW, ex = sexp + rs * C::EXP;
+      if (!mbar_wait_warp(bar(16 + rs), (j / C::NR) & 1, abort, ST_TIMEOUT_ATTN)) break;
+      // exponents of keys 2 lane, 2 lane + 1; NaN rows and keys that do not exist take no part in the maxima
+      const bool even_ok = (sgran[rs] >> (lane >> 3)) & 1u && c0 + j * PF_BN + 2 * lane < c1;
+      const bool odd_ok = even_ok && c0 + j * PF_BN + 2 * lane + 1 < c1;
+      const uint32_t kb = ld_shared_u16(ex + 2 * lane), vb = ld_shared_u16(ex + PF_BN + 2 * lane);
+      const int k2[2] = {(int)(kb & 255u), (int)(kb >> 8)}, v2[2] = {(int)(vb & 255u), (int)(vb >> 8)};
       int kn = 0, vn = 0;
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        if ((e ? x.odd : x.even) && k2[e] != 255 && v2[e] != 255) kn = max(kn, k2[e]), vn = max(vn, v2[e]);
+        if ((e ? odd_ok : even_ok) && k2[e] != 255 && v2[e] != 255) kn = max(kn, k2[e]), vn = max(vn, v2[e]);
       kn = __reduce_max_sync(0xffffffffu, kn);
       vn = __reduce_max_sync(0xffffffffu, vn);
-      const uint32_t even = __ballot_sync(0xffffffffu, x.even), odd = __ballot_sync(0xffffffffu, x.odd);
-      const uint32_t kp = __shfl_sync(0xffffffffu, x.kbytes, row >> 1), vp = __shfl_sync(0xffffffffu, x.vbytes, row >> 1);
+      const uint32_t even = __ballot_sync(0xffffffffu, even_ok), odd = __ballot_sync(0xffffffffu, odd_ok);
+      const uint32_t kp = __shfl_sync(0xffffffffu, kb, row >> 1), vp = __shfl_sync(0xffffffffu, vb, row >> 1);
       const int nk = row & 1 ? kp >> 8 : kp & 255u, nv = row & 1 ? vp >> 8 : vp & 255u;
-      const bool nan = nk == 255 || nv == 255;
-      if (!mbar_wait_warp(bar(4 + s), par, abort, ST_TIMEOUT_ATTN)) return false;
-      put(sk + s * C::KV_BYTES, x.kx, nan ? 0xffffffffu : scale_of(nk, kn), 0x7e007e00u);
+      const bool none = nk == 255 || nv == 255 || !(((row & 1 ? odd : even) >> (row >> 1)) & 1u);
+      if (!mbar_wait_warp(bar(4 + s), par, abort, ST_TIMEOUT_ATTN)) break;
+      put(sk + s * C::KV_BYTES, raw, none ? 0xffffffffu : scale_of(nk, kn), 0x7e007e00u);  // NaN where there is no key either: masked
       if (lane == 0) mbar_arrive(bar(s));
-      if (!mbar_wait_warp(bar(6 + s), par, abort, ST_TIMEOUT_ATTN)) return false;
-      put(sv + s * C::KV_BYTES, x.vx, nan ? 0xffffffffu : scale_of(nv, vn), 0u);
+      if (!mbar_wait_warp(bar(6 + s), par, abort, ST_TIMEOUT_ATTN)) break;
+      put(sv + s * C::KV_BYTES, raw + PF_BN * D, none ? 0xffffffffu : scale_of(nv, vn), 0u);
       if (w == 0 && lane == 0) {
         skn[s] = kn - 127;
         svn[s] = vn - 127;
@@ -193,21 +168,45 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
         sodd[s] = odd;
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(2 + s));
-      return true;
-    };
-    // two tiles in registers: the next one's bytes arrive while this one is converted
-    Tile x0, x1;
-    pages(0);
-    load(0, x0);
-    for (int j = 0; j < ntiles; j += 2) {
-      if (j + 1 < ntiles) load(j + 1, x1);
-      if (!convert(j, x0)) break;
-      if (j + 1 < ntiles) {
-        if (j + 2 < ntiles) load(j + 2, x0);
-        if (!convert(j + 1, x1)) break;
+      if (lane == 0) {
+        mbar_arrive(bar(2 + s));
+        mbar_arrive(bar(20 + rs));
       }
     }
+  } else if (warp == 13) {  // --------------------------------------------------------------------- copies
+    // lanes 0-3: K rows of a group of 16 keys, 4-7: V rows, 8-11 and 12-15: their exponents
+    const int gr = lane & 3, what = (lane >> 2) & 3;
+    const uint8_t* src = what == 0 ? a.kc + h * a.cH : what == 1 ? a.vc + h * a.cH : what == 2 ? a.ke + h * a.eH : a.ve + h * a.eH;
+    const long long pstride = what < 2 ? a.cP : a.eP;
+    const int each = what < 2 ? D : 1;  // bytes per key
+    CopyLedger ledger;
+    int off = 0;
+    auto page_of = [&](int j) {
+      const int key = c0 + j * PF_BN + gr * 16, pi = a.shift >= 0 ? key >> a.shift : key / a.page;
+      off = key - pi * a.page;
+      return key < c1 ? a.prefix[pi] : -1;
+    };
+    int id = page_of(0);
+    for (int j = 0; j < ntiles; ++j) {
+      const int s = j % C::NR;
+      const bool ok = id >= 0 && id < a.pages;
+      if (!ok && c0 + j * PF_BN + gr * 16 < c1) record_status(ST_BAD_PAGE);
+      const uint8_t* from = src + (ok ? id : 0) * pstride + (long long)off * each;
+      if (j + 1 < ntiles) id = page_of(j + 1);
+      if (!mbar_wait_warp(bar(20 + s), ((j / C::NR) & 1) ^ 1, abort, ST_TIMEOUT_ATTN)) break;
+      const uint32_t groups = __ballot_sync(0xffffffffu, ok) & 15u;
+      if (lane == 0) {
+        sgran[s] = groups;
+        ledger.arm(s, (j / C::NR) & 1);
+        mbar_arrive_expect_tx(bar(16 + s), __popc(groups) * 2 * 16 * (D + 1));
+      }
+      __syncwarp();
+      if (ok && lane < 16)
+        bulk_load(what < 2 ? sraw + s * C::RAW + (what * PF_BN + gr * 16) * D : sexp + s * C::EXP + (what - 2) * PF_BN + gr * 16, from,
+                  16 * each, bar(16 + s));
+    }
+    if (lane == 0) ledger.drain([&](int i) { return bar(16 + i); });  // no copy outlives the CTA
+    __syncwarp();
   } else if (warp == 12) {  // --------------------------------------------------------------------- MMA issue
     if (lane == 0) {
       constexpr uint32_t IDESC_S = idesc_f16(PF_ROWS, PF_BN), IDESC_PV = idesc_f16(PF_ROWS, D, /*b_mn_major=*/1);
