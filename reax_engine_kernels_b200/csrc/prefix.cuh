@@ -64,8 +64,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
   __shared__ uint32_t sgran[4];  // which of a raw tile's four groups of 16 keys were copied
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
-  __shared__ int skn[2], svn[2];            // a tile's largest nk and nv
-  __shared__ uint32_t seven[2], sodd[2];    // its even and odd keys that exist
+  __shared__ int skn[4], svn[4];          // a tile's largest nk and nv
+  __shared__ uint32_t seven[4], sodd[4];  // its even and odd keys that exist
   pdl_launch();  // the own keys' kernel needs nothing from here
   const uint32_t base = (smem_u32(pf_raw) + 1023u) & ~1023u;
   const uint32_t sk = base, sv = sk + 2 * C::KV_BYTES, sraw = sv + 2 * C::KV_BYTES, sexp = sraw + C::NR * C::RAW;
@@ -98,33 +98,33 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
   volatile int* abort = &abort_flag;
 
   if (warp >= 4 && warp < 12) {  // ---------------------------------------------------------------- dequantisation
-    // a load of a warp covers whole rows: LPR lanes a row, its unit i rows RPU i .. + RPU - 1 of the warp's eight
-    constexpr int LPR = D / 16, RPU = 32 / LPR, U = 8 / RPU;
-    const int w = warp - 4, row = w * 8 + (lane & 7), sub = lane % LPR, ur = lane / LPR;
-    const bool swap = (sub >> 2) & 1;  // which half goes first, so that eight lanes' stores fall in different banks
+    // A load of a warp covers whole rows, two (D = 256) or four, 64 bytes to four lanes.  Neighbouring groups of four lanes take
+    // neighbouring rows and different 64-byte parts, so that eight lanes' loads and stores fall in different banks.
+    constexpr int RPU = 512 / D, U = 8 / RPU, NQ = D / 64;
+    const int w = warp - 4, row = w * 8 + (lane & 7), grp = lane >> 2;
+    const int ur = 2 * ((grp >> 1) / NQ) + (grp & 1), quad = ((grp >> 1) + (grp & 1)) % NQ;
     // scale: of row w * 8 + (lane & 7); all ones: a row without values, filled with `fill`
     auto put = [&](uint32_t buf, uint32_t raw, uint32_t scale, uint32_t fill) {
       uint4 x[U];
 #pragma unroll
-      for (int i = 0; i < U; ++i) x[i] = ld_shared_v4(raw + (w * 8 + i * RPU) * D + lane * 16);
+      for (int i = 0; i < U; ++i) x[i] = ld_shared_v4(raw + (w * 8 + i * RPU + ur) * D + quad * 64 + (lane & 3) * 16);
+      const bool some = __any_sync(0xffffffffu, scale == 0xffffffffu);
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        const int r = i * RPU + ur, c = 2 * sub;  // first of two 16-byte chunks of the f16 row
+        const int r = i * RPU + ur;
         const uint32_t sc = __shfl_sync(0xffffffffu, scale, r);
-        const bool none = sc == 0xffffffffu;
-        const uint32_t mul = none ? 0u : sc, add = none ? fill : 0u, keep = none ? 0u : 0xffffffffu;
-        const uint32_t y[4] = {(swap ? x[i].z : x[i].x) & keep, (swap ? x[i].w : x[i].y) & keep, (swap ? x[i].x : x[i].z) & keep,
-                               (swap ? x[i].y : x[i].w) & keep};
-        const uint32_t dst = buf + (c >> 3) * (PF_BN * 128) + (w * 8 + r) * 128;
+        const uint32_t y[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+        const uint32_t dst = buf + quad * (PF_BN * 128) + (w * 8 + r) * 128;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           uint32_t z[4];
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
             const uint32_t v = e4m3x2_f16x2((uint16_t)(n & 1 ? y[2 * k + (n >> 1)] >> 16 : y[2 * k + (n >> 1)]));
-            asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(z[n]) : "r"(v), "r"(mul), "r"(add));
+            asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(z[n]) : "r"(v), "r"(sc));
           }
-          st_shared_v4(dst + (((((c & 7) + k) ^ (int)swap) ^ r) << 4), make_uint4(z[0], z[1], z[2], z[3]));
+          if (some && sc == 0xffffffffu) z[0] = z[1] = z[2] = z[3] = fill;
+          st_shared_v4(dst + (((2 * (lane & 3) + k) ^ r) << 4), make_uint4(z[0], z[1], z[2], z[3]));
         }
       }
       fence_proxy_async_smem();
@@ -158,16 +158,17 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
       const bool none = nk == 255 || nv == 255 || !(((row & 1 ? odd : even) >> (row >> 1)) & 1u);
       if (!mbar_wait_warp(bar(4 + s), par, abort, ST_TIMEOUT_ATTN)) break;
       put(sk + s * C::KV_BYTES, raw, none ? 0xffffffffu : scale_of(nk, kn), 0x7e007e00u);  // NaN where there is no key either: masked
+      // For the softmax, which reads it after S_j.  Four of them: this one's place was read by the softmax of j - 4, which was done
+      // before S_{j-2} was issued, whose end K_j's buffer waited for.
+      if (w == 0 && lane == 0) {
+        skn[j & 3] = kn - 127;
+        svn[j & 3] = vn - 127;
+        seven[j & 3] = even;
+        sodd[j & 3] = odd;
+      }
       if (lane == 0) mbar_arrive(bar(s));
       if (!mbar_wait_warp(bar(6 + s), par, abort, ST_TIMEOUT_ATTN)) break;
       put(sv + s * C::KV_BYTES, raw + PF_BN * D, none ? 0xffffffffu : scale_of(nv, vn), 0u);
-      if (w == 0 && lane == 0) {
-        skn[s] = kn - 127;
-        svn[s] = vn - 127;
-        seven[s] = even;
-        sodd[s] = odd;
-      }
-      __syncwarp();
       if (lane == 0) {
         mbar_arrive(bar(2 + s));
         mbar_arrive(bar(20 + rs));
@@ -286,15 +287,14 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
     bool live = true;
     for (int j = 0; j < ntiles; ++j) {
       const int s = j & 1;
-      live = mbar_wait_warp(bar(8 + s), (j >> 1) & 1, abort, ST_TIMEOUT_ATTN) &&
-             mbar_wait_warp(bar(2 + s), (j >> 1) & 1, abort, ST_TIMEOUT_ATTN);  // the tile's exponents come with V
+      live = mbar_wait_warp(bar(8 + s), (j >> 1) & 1, abort, ST_TIMEOUT_ATTN);
       if (!live) break;
       tc_fence_after();
       uint32_t x[64];
       tmem_ld64(lanes + s * 64, x);
-      const int k0 = c0 + j * PF_BN, vn = svn[s];
-      const uint32_t even = seven[s], odd = sodd[s];
-      float c1s = rs * pow2_byte((uint32_t)(skn[s] + 127));
+      const int k0 = c0 + j * PF_BN, vn = svn[j & 3];
+      const uint32_t even = seven[j & 3], odd = sodd[j & 3];
+      float c1s = rs * pow2_byte((uint32_t)(skn[j & 3] + 127));
       if (c1s < 0x1p-126f) c1s = 0x1p-126f;  // not 0: a masked score is -inf
       if (__any_sync(0xffffffffu, k0 + PF_BN - 1 > lim || (even & odd) != 0xffffffffu)) {
 #pragma unroll
