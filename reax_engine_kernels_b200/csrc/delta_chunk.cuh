@@ -15,16 +15,18 @@
 // Bound: the tensor pipe of mma.sync.  A warp owns 16 rows of h in accumulator fragments (64 registers), which are at once
 // the layout of the A operand of h k, so the state never leaves the registers; 310 m16n8k16 per warp and chunk, 8 cycles
 // each.  (tcgen05 would want 128 rows and the state in tensor memory, to be read, split and written back each chunk; three
-// bf16 terms at 16 rows keep it in place.)  A CTA is 64 rows of one (sequence, head): four such warps, and two that
-// prepare the next chunk (copies, the two Gram matrices, decays, the triangular inverse) while the four work on
-// this one, with one barrier per chunk.  Two CTAs per SM.
+// bf16 terms at 16 rows keep it in place.)  A CTA is 64 rows of one (sequence, head): four such warps, and four that
+// prepare the next chunk (the two Gram matrices, decays, the triangular inverse) while the four work on this one, with one
+// barrier per chunk for all.  The two groups of four split the registers 168 / 88 (setmaxnreg), and two CTAs fit an SM.
+// With two preparing warps, each with a whole Gram matrix and its own decays, the preparation took 8000 cycles a chunk
+// against the products' 4000 to 5800.
 #pragma once
 #include "delta_state.cuh"
 
 namespace reax {
 
 constexpr int DC_T = 32;                 // tokens per chunk
-constexpr int DC_THREADS = 192;
+constexpr int DC_THREADS = 256;
 constexpr int DC_KP = 272, DC_VP = 144;  // row pitches in bytes of k, q and of v: 16 past a multiple of 128, so that eight rows of an
 constexpr int DC_MP = 80;                // ldmatrix fall in different banks; of T and of P (32 bf16)
 struct DcIn {                            // a chunk's inputs
@@ -32,14 +34,16 @@ struct DcIn {                            // a chunk's inputs
 };
 struct DcPrep {  // what is prepared of them
   uint8_t T[3][DC_T * DC_MP], P[2][DC_T * DC_MP];
-  float grow[DC_T], left[DC_T];  // 2^G_i, 2^(G_last - G_i)
 };
 struct DcSmem {
   DcIn in[3];
   DcPrep prep[2];
-  long long G[2][DC_T];
-  float L[DC_T][DC_T + 4];  // column by column
-  float beta[DC_T];
+  struct {
+    int whole[DC_T];   // G_i = whole + frac, 0 <= frac < 1
+    float frac[DC_T], beta[DC_T];
+    float grow[DC_T], left[DC_T];  // 2^G_i, 2^(G_last - G_i)
+  } G[3];                          // chunk c's in c % 3
+  float L[DC_T][DC_T + 4];  // column by column; then the inverse, row by row
   uint8_t o[4][DC_T * 48];  // per warp: 32 tokens x 16 rows
 };
 
@@ -89,110 +93,107 @@ __device__ __forceinline__ void split_frag(const float (&c0)[4], const float (&c
   }
 }
 
-// copies of the 32 tokens from t on into `in`, zeros past the sequence's end; all threads
-__device__ __forceinline__ void dc_load(const DeltaArgs& a, DcIn& in, long long t, long long e, int hk, int hv, int row0) {
+// copies of the 32 tokens from t on into `in`, zeros past the sequence's end; the 128 preparing threads
+__device__ __forceinline__ void dc_load(const DeltaArgs& a, DcIn& in, long long t, long long e, int hk, int hv, int row0, int pt) {
   const int kT = a.H * 128, vT = a.HV * 128, left = (int)min(e - t, (long long)DC_T);
   const uint16_t *k = a.k + t * kT + hk * 128, *q = a.q + t * kT + hk * 128, *v = a.v + t * vT + hv * 128 + row0;
 #pragma unroll
-  for (int i = 0; i < (DC_T * 16 + DC_THREADS - 1) / DC_THREADS; ++i) {
-    const int x = threadIdx.x + i * DC_THREADS, r = x >> 4, c = x & 15;
-    if (x < DC_T * 16) {
-      const int off = (r < left ? r : 0) * kT + c * 8;
-      cp_async16(smem_u32(in.k + r * DC_KP + c * 16), k + off, r < left);
-      cp_async16(smem_u32(in.q + r * DC_KP + c * 16), q + off, r < left);
-    }
+  for (int i = 0; i < DC_T * 16 / 128; ++i) {
+    const int x = pt + i * 128, r = x >> 4, c = x & 15;
+    const int off = (r < left ? r : 0) * kT + c * 8;
+    cp_async16(smem_u32(in.k + r * DC_KP + c * 16), k + off, r < left);
+    cp_async16(smem_u32(in.q + r * DC_KP + c * 16), q + off, r < left);
   }
 #pragma unroll
-  for (int i = 0; i < (DC_T * 8 + DC_THREADS - 1) / DC_THREADS; ++i) {
-    const int x = threadIdx.x + i * DC_THREADS, r = x >> 3, c = x & 7;
-    if (x < DC_T * 8) cp_async16(smem_u32(in.v + r * DC_VP + c * 16), v + (r < left ? r : 0) * vT + c * 8, r < left);
+  for (int i = 0; i < DC_T * 8 / 128; ++i) {
+    const int x = pt + i * 128, r = x >> 3, c = x & 7;
+    cp_async16(smem_u32(in.v + r * DC_VP + c * 16), v + (r < left ? r : 0) * vT + c * 8, r < left);
   }
 }
 
-// 2^(x / 2^32): the fraction by ex2, the whole part into the exponent (0 below fp32's normal range, infinity above its range)
-__device__ __forceinline__ float exp2_fixed(long long x) {
-  const int whole = (int)(x >> 32);
-  const float f = ex2_approx((float)((uint32_t)x >> 8) * 0x1p-24f);  // in [1, 2): 24 bits of the fraction are exact in fp32
-  return whole < -126 ? 0.f : whole > 127 ? INFINITY : __uint_as_float(__float_as_uint(f) + ((uint32_t)whole << 23));
+// 2^(whole + frac) for whole < 2^23, |frac| < 1, the whole part into ex2's exponent: 0 where it would pass 2^-126, not above 2^126
+__device__ __forceinline__ float exp2_parts(int whole, float frac) {
+  return __uint_as_float(__float_as_uint(ex2_approx(frac)) + ((uint32_t)min(max(whole, -125), 125) << 23)) * (whole < -125 ? 0.f : 1.f);
 }
 
-// One of the two preparing warps: w = 0 the inverse T (from k . k), w = 1 the products P (from q . k) and the decays.
-__device__ __forceinline__ void dc_prepare(DcSmem& s, const DcIn& in, DcPrep& out, int w, int lane, float g, float beta) {
-  const int gq = lane >> 2, t = lane & 3;
-  // G_i.  Past +-2^9 a token's decay is 0 or infinite in fp32 anyway; a NaN one makes its beta NaN
-  const float gc = fminf(fmaxf(g, -512.f), 512.f);
-  long long G = __float2ll_rn(gc * 0x1p32f);
+// The decays of a chunk, a token per lane: G and beta for the Gram matrices, 2^G_i and 2^(G_last - G_i) for the products.
+__device__ __forceinline__ void dc_decays(DcSmem& s, int slot, int lane, float g, float beta) {
+  // Past +-2^9 a token's decay is 0 or infinite in fp32 anyway; a NaN one makes its beta NaN
+  long long G = __float2ll_rn(fminf(fmaxf(g, -512.f), 512.f) * 0x1p32f);
   if (g != g) beta = g;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const long long x = __shfl_up_sync(0xffffffffu, G, o);
     if (lane >= o) G += x;
   }
-  s.G[w][lane] = G;
-  if (w == 1) {
-    out.grow[lane] = exp2_fixed(G);
-    out.left[lane] = exp2_fixed(__shfl_sync(0xffffffffu, G, 31) - G);
-  } else {
-    s.beta[lane] = beta;
-  }
-  __syncwarp();
-  // rows i of k (or q) times rows j of k, tiles that touch the lower triangle
-  const uint32_t ka = smem_u32(in.k), xa = w ? smem_u32(in.q) : ka;
-  float acc[2][4][4];
+  const int whole = (int)(G >> 32);
+  const float frac = (float)((uint32_t)G >> 8) * 0x1p-24f;  // 24 bits are exact
+  s.G[slot].whole[lane] = whole;
+  s.G[slot].frac[lane] = frac;
+  s.G[slot].beta[lane] = beta;
+  s.G[slot].grow[lane] = exp2_parts(whole, frac);
+  s.G[slot].left[lane] = exp2_parts(__shfl_sync(0xffffffffu, whole, 31) - whole, __shfl_sync(0xffffffffu, frac, 31) - frac);
+}
+
+// A third of both Gram matrices: w = 0 rows 0-15 by columns 0-15, 1 rows 16-31 by columns 0-15, 2 rows 16-31 by columns 16-31.
+// L = -(strictly lower beta_i 2^(G_i - G_j) k_i . k_j) to s.L, P = lower 2^(G_i - G_j) q_i . k_j in two terms.
+__device__ __forceinline__ void dc_gram(DcSmem& s, const DcIn& in, int slot, DcPrep& out, int w, int lane) {
+  const int gq = lane >> 2, t = lane & 3, i0 = w ? 16 : 0, j0 = w == 2 ? 16 : 0;
+  const uint32_t ka = smem_u32(in.k), qa = smem_u32(in.q);
+  float acc[2][2][4];  // k . k, q . k; column tiles
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int n = 0; n < 4; ++n)
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.f;
+  const uint32_t arow = (i0 + (lane & 15)) * DC_KP + (lane >> 4) * 16, brow = (j0 + (lane & 7) + (lane >> 4) * 8) * DC_KP + ((lane >> 3) & 1) * 16;
 #pragma unroll
   for (int ks = 0; ks < 8; ++ks) {
-    uint32_t x[2][4], b[2][4];
+    uint32_t x[2][4], b[4];
+    ldsm_x4(ka + arow + ks * 32, x[0]);
+    ldsm_x4(qa + arow + ks * 32, x[1]);
+    ldsm_x4(ka + brow + ks * 32, b);
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-      ldsm_x4(xa + (m * 16 + (lane & 15)) * DC_KP + ks * 32 + (lane >> 4) * 16, x[m]);
-      ldsm_x4(ka + (m * 16 + (lane & 7) + (lane >> 4) * 8) * DC_KP + ks * 32 + ((lane >> 3) & 1) * 16, b[m]);
+      mma_bf16(acc[m][0], x[m], b[0], b[1]);
+      mma_bf16(acc[m][1], x[m], b[2], b[3]);
     }
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-      for (int n = 0; n < 2 * (m + 1); ++n) mma_bf16(acc[m][n], x[m], b[n >> 1][(n & 1) * 2], b[n >> 1][(n & 1) * 2 + 1]);
   }
-  long long Gi[2][2], Gj[4][2];  // all read before the first store below, which the compiler would not move them across
-  float bi[2][2];
+  int Wi[2], Wj[2][2];
+  float Fi[2], Fj[2][2], bi[2];  // all read before the first store below, which the compiler would not move them across
 #pragma unroll
-  for (int m = 0; m < 4; ++m) {
-    const longlong2 x = *reinterpret_cast<const longlong2*>(&s.G[w][m * 8 + 2 * t]);
-    Gj[m][0] = x.x, Gj[m][1] = x.y;
-    Gi[m >> 1][m & 1] = s.G[w][m * 8 + gq];
-    bi[m >> 1][m & 1] = s.beta[m * 8 + gq];
+  for (int r = 0; r < 2; ++r) {
+    const int i = i0 + gq + 8 * r, j = j0 + 8 * r + 2 * t;
+    Wi[r] = s.G[slot].whole[i], Fi[r] = s.G[slot].frac[i], bi[r] = -s.G[slot].beta[i];
+    const int2 wj = *reinterpret_cast<const int2*>(&s.G[slot].whole[j]);
+    const float2 fj = *reinterpret_cast<const float2*>(&s.G[slot].frac[j]);
+    Wj[r][0] = wj.x, Wj[r][1] = wj.y, Fj[r][0] = fj.x, Fj[r][1] = fj.y;
   }
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+  for (int n = 0; n < 2; ++n)
 #pragma unroll
-    for (int n = 0; n < 2 * (m + 1); ++n)
+    for (int r = 0; r < 2; ++r) {
+      const int i = i0 + gq + 8 * r, j = j0 + n * 8 + 2 * t;
+      float d[2], p[2];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int i = m * 16 + gq + 8 * r, j = n * 8 + 2 * t;
-        float x[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float d = acc[m][n][2 * r + e] * exp2_fixed(Gi[m][r] - Gj[n][e]);
-          x[e] = (w ? j + e <= i : j + e < i) ? d : 0.f;
-        }
-        if (w) {
-          uint32_t p[2];
-          split_bf16<2>(x[0], x[1], p);
-#pragma unroll
-          for (int k = 0; k < 2; ++k) *reinterpret_cast<uint32_t*>(out.P[k] + i * DC_MP + j * 2) = p[k];
-        } else {
-          s.L[j][i] = -bi[m][r] * x[0];
-          s.L[j + 1][i] = -bi[m][r] * x[1];
-        }
+      for (int e = 0; e < 2; ++e) {
+        const float x = exp2_parts(Wi[r] - Wj[n][e], Fi[r] - Fj[n][e]);
+        d[e] = j + e < i ? bi[r] * (acc[0][n][2 * r + e] * x) : 0.f;
+        p[e] = j + e <= i ? acc[1][n][2 * r + e] * x : 0.f;
       }
-  if (w) return;
-  __syncwarp();
-  // column `lane` of (1 + L)^-1 by forward substitution, right-looking: once x_j is final, it leaves the later ones
+      s.L[j][i] = d[0];
+      s.L[j + 1][i] = d[1];
+      uint32_t y[2];
+      split_bf16<2>(p[0], p[1], y);
+      *reinterpret_cast<uint32_t*>(out.P[0] + i * DC_MP + j * 2) = y[0];
+      *reinterpret_cast<uint32_t*>(out.P[1] + i * DC_MP + j * 2) = y[1];
+    }
+}
+
+// One warp: column `lane` of (1 + L)^-1 by forward substitution, right-looking: once x_j is final, it leaves the later ones.  Over
+// s.L, row by row.
+__device__ __forceinline__ void dc_inverse(DcSmem& s, int lane) {
   float x[DC_T];
 #pragma unroll
   for (int i = 0; i < DC_T; ++i) x[i] = i == lane ? 1.f : 0.f;
@@ -200,29 +201,72 @@ __device__ __forceinline__ void dc_prepare(DcSmem& s, const DcIn& in, DcPrep& ou
   for (int j = 0; j < DC_T - 1; ++j)
 #pragma unroll
     for (int i = (j + 1) & ~3; i < DC_T; i += 4) {
-      const float4 l = *reinterpret_cast<const float4*>(&s.L[j][i]);  // L is strictly lower: what lies above is not used
+      const float4 l = *reinterpret_cast<const float4*>(&s.L[j][i]);  // what lies on and above the diagonal is not used
       if (i > j) x[i] = __fmaf_rn(l.x, x[j], x[i]);
       if (i + 1 > j) x[i + 1] = __fmaf_rn(l.y, x[j], x[i + 1]);
       if (i + 2 > j) x[i + 2] = __fmaf_rn(l.z, x[j], x[i + 2]);
       x[i + 3] = __fmaf_rn(l.w, x[j], x[i + 3]);
     }
+  __syncwarp();  // every lane has read L
 #pragma unroll
-  for (int i = 0; i < DC_T; ++i) {
-    float y = x[i] * beta;
+  for (int i = 0; i < DC_T; ++i) s.L[i][lane] = x[i];
+}
+
+// T = inverse * beta_j in three terms; thread pt of the 128 takes 8 columns of a row
+__device__ __forceinline__ void dc_terms(const DcSmem& s, int slot, DcPrep& out, int pt) {
+  const int i = pt >> 2, j = (pt & 3) * 8;
+  uint32_t y[3][4];
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      const uint16_t b = __bfloat16_as_ushort(__float2bfloat16_rn(y));
-      *reinterpret_cast<uint16_t*>(out.T[k] + i * DC_MP + lane * 2) = b;
-      y -= bf_lo(b);
-    }
+  for (int c = 0; c < 4; ++c) {
+    const float2 x = *reinterpret_cast<const float2*>(&s.L[i][j + 2 * c]), b = *reinterpret_cast<const float2*>(&s.G[slot].beta[j + 2 * c]);
+    uint32_t z[3];
+    split_bf16<3>(x.x * b.x, x.y * b.y, z);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) y[k][c] = z[k];
   }
+#pragma unroll
+  for (int k = 0; k < 3; ++k)
+    *reinterpret_cast<uint4*>(out.T[k] + i * DC_MP + j * 2) = make_uint4(y[k][0], y[k][1], y[k][2], y[k][3]);
+}
+
+// The four preparing warps, chunk c (its decays are there already), and warp 3 the decays of c + 1
+template <typename Decays>
+__device__ __forceinline__ void dc_prepare(DcSmem& s, int c, int w, int lane, Decays decays) {
+  DcPrep& out = s.prep[c & 1];
+  if (w < 3) dc_gram(s, s.in[c % 3], c % 3, out, w, lane);
+  named_bar_sync<1, 128>();
+  if (w == 3) dc_inverse(s, lane);
+  named_bar_sync<1, 128>();
+  dc_terms(s, c % 3, out, w * 32 + lane);
+  if (w == 3) decays();
+}
+
+// The sequence of this CTA: the longest first (they are the last to end), in their order past a length that one pass can sort.
+__device__ __forceinline__ int dc_sequence(const DeltaArgs& a) {
+  __shared__ long long len[DC_THREADS];
+  __shared__ int mine;
+  if (a.N > DC_THREADS) return blockIdx.z;
+  const int i = threadIdx.x;
+  if (i < a.N) {
+    long long b, e;
+    delta_range(a, i, b, e);
+    len[i] = e - b;
+  }
+  __syncthreads();
+  if (i < a.N) {
+    int before = 0;
+    for (int k = 0; k < a.N; ++k) before += len[k] > len[i] || (len[k] == len[i] && k < i);
+    if (before == (int)blockIdx.z) mine = i;
+  }
+  __syncthreads();
+  return mine;
 }
 
 // grid (2, HV, N): 64 rows of one (sequence, value head) per CTA; sequences of at most DS_MOST tokens are the step kernel's
 __global__ void __launch_bounds__(DC_THREADS, 2) delta_chunk_kernel(DeltaArgs a) {
   extern __shared__ __align__(128) uint8_t dc_raw[];
   DcSmem& s = *reinterpret_cast<DcSmem*>(dc_raw);
-  const int n = blockIdx.z, hv = blockIdx.y, lane = threadIdx.x & 31, warp = warp_id();
+  const int n = dc_sequence(a), hv = blockIdx.y, lane = threadIdx.x & 31, warp = warp_id();
   const int gq = lane >> 2, t4 = lane & 3, row0 = blockIdx.x * 64;
   long long t0, e;
   delta_range(a, n, t0, e);
@@ -237,28 +281,42 @@ __global__ void __launch_bounds__(DC_THREADS, 2) delta_chunk_kernel(DeltaArgs a)
   }
   const int hk = hv / (a.HV / a.H);
   const int chunks = (int)((e - t0 + DC_T - 1) / DC_T);
-  float gw = 0.f;  // the preparing lanes' token's decay and beta (still as bits: a conversion would wait for it), a chunk ahead
-  uint16_t bw = 0;
-  auto scalars = [&](int c) {
-    const long long t = t0 + (long long)c * DC_T + lane;
-    gw = t < e ? a.g[t * a.HV + hv] : 0.f;
-    bw = t < e ? a.beta[t * a.HV + hv] : (uint16_t)0;
-  };
-
-  float h[16][4];
-  dc_load(a, s.in[0], t0, e, hk, hv, row0);
-  cp_async_commit();
-  if (chunks > 1) dc_load(a, s.in[1], t0 + DC_T, e, hk, hv, row0);
-  cp_async_commit();
-  if (warp >= 4) scalars(0);
-  cp_async_wait<1>();
-  __syncthreads();
+  // The two roles' loops meet at one barrier per chunk: chunk c + 1 is prepared while the products of c run
   if (warp >= 4) {
-    const float g = gw, b = bf_lo(bw);
-    scalars(1);
-    dc_prepare(s, s.in[0], s.prep[0], warp - 4, lane, g, b);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    const int pt = threadIdx.x - 128;
+    // warp 7: its lanes' token's decay and beta of chunk c, asked for well before the decays are computed
+    float gw = 0.f;
+    uint16_t bw = 0;  // still as bits: a conversion would wait for it
+    auto scalars = [&](int c) {
+      const long long t = t0 + (long long)c * DC_T + lane;
+      gw = t < e ? a.g[t * a.HV + hv] : 0.f;
+      bw = t < e ? a.beta[t * a.HV + hv] : (uint16_t)0;
+    };
+    dc_load(a, s.in[0], t0, e, hk, hv, row0, pt);
+    cp_async_commit();
+    if (warp == 7) {
+      scalars(0);
+      dc_decays(s, 0, lane, gw, bf_lo(bw));
+      scalars(1);
+    }
+    cp_async_wait<0>();
+    named_bar_sync<1, 128>();
+    for (int c = -1; c < chunks; ++c) {
+      if (c + 2 < chunks) dc_load(a, s.in[(c + 2) % 3], t0 + (long long)(c + 2) * DC_T, e, hk, hv, row0, pt);
+      cp_async_commit();
+      if (c + 1 < chunks)
+        dc_prepare(s, c + 1, warp - 4, lane, [&] {
+          dc_decays(s, (c + 2) % 3, lane, gw, bf_lo(bw));
+          scalars(c + 3);
+        });
+      cp_async_wait<0>();
+      named_bar_sync<2, DC_THREADS>();
+    }
   } else {
-    const float* st = a.state + slot * a.sS + ((long long)hv * 128 + row0 + warp * 16 + gq) * 128 + 2 * t4;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    float h[16][4];
+    float* st = a.state + slot * a.sS + ((long long)hv * 128 + row0 + warp * 16 + gq) * 128 + 2 * t4;
     const bool fresh = a.fresh && a.fresh[n];
 #pragma unroll
     for (int j = 0; j < 16; ++j)
@@ -268,22 +326,11 @@ __global__ void __launch_bounds__(DC_THREADS, 2) delta_chunk_kernel(DeltaArgs a)
         h[j][2 * r] = x.x;
         h[j][2 * r + 1] = x.y;
       }
-  }
-  cp_async_wait<0>();
-  __syncthreads();
-
-  for (int c = 0; c < chunks; ++c) {
-    if (c + 2 < chunks) dc_load(a, s.in[(c + 2) % 3], t0 + (long long)(c + 2) * DC_T, e, hk, hv, row0);
-    cp_async_commit();
-    if (warp >= 4) {
-      if (c + 1 < chunks) {
-        const float g = gw, b = bf_lo(bw);
-        scalars(c + 2);
-        dc_prepare(s, s.in[(c + 1) % 3], s.prep[(c + 1) & 1], warp - 4, lane, g, b);
-      }
-    } else {
+    named_bar_sync<2, DC_THREADS>();
+    for (int c = 0; c < chunks; ++c) {
       const DcIn& in = s.in[c % 3];
       const DcPrep& pr = s.prep[c & 1];
+      const auto& dec = s.G[c % 3];
       const uint32_t ka = smem_u32(in.k), qa = smem_u32(in.q), va = smem_u32(in.v);
       // ---- h k (three terms) and h q (two)
       float sk[4][4], sq[4][4];
@@ -321,7 +368,7 @@ __global__ void __launch_bounds__(DC_THREADS, 2) delta_chunk_kernel(DeltaArgs a)
         ldsm_x4_t(vaddr + p * 16 * DC_VP, vv);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const float2 gr = *reinterpret_cast<const float2*>(&pr.grow[(2 * p + x) * 8 + 2 * t4]);
+          const float2 gr = *reinterpret_cast<const float2*>(&dec.grow[(2 * p + x) * 8 + 2 * t4]);
           float(&k4)[4] = sk[2 * p + x];
           float(&q4)[4] = sq[2 * p + x];
 #pragma unroll
@@ -392,7 +439,7 @@ __global__ void __launch_bounds__(DC_THREADS, 2) delta_chunk_kernel(DeltaArgs a)
         dst[1] = *reinterpret_cast<const uint4*>(s.o[warp] + lane * 48 + 16);
       }
       // ---- h <- 2^G_last h + (2^(G_last - G_j) u_j) k_j^T
-      const float last = pr.grow[DC_T - 1];
+      const float last = dec.grow[DC_T - 1];
 #pragma unroll
       for (int j = 0; j < 16; ++j)
 #pragma unroll
@@ -401,7 +448,7 @@ __global__ void __launch_bounds__(DC_THREADS, 2) delta_chunk_kernel(DeltaArgs a)
       for (int ks = 0; ks < 2; ++ks) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const float2 le = *reinterpret_cast<const float2*>(&pr.left[(2 * ks + x) * 8 + 2 * t4]);
+          const float2 le = *reinterpret_cast<const float2*>(&dec.left[(2 * ks + x) * 8 + 2 * t4]);
           float(&u4)[4] = u[2 * ks + x];
           u4[0] *= le.x, u4[1] *= le.y, u4[2] *= le.x, u4[3] *= le.y;
         }
@@ -418,12 +465,8 @@ __global__ void __launch_bounds__(DC_THREADS, 2) delta_chunk_kernel(DeltaArgs a)
           }
         }
       }
+      named_bar_sync<2, DC_THREADS>();
     }
-    cp_async_wait<0>();
-    __syncthreads();
-  }
-  if (warp < 4) {
-    float* st = a.state + slot * a.sS + ((long long)hv * 128 + row0 + warp * 16 + gq) * 128 + 2 * t4;
 #pragma unroll
     for (int j = 0; j < 16; ++j)
 #pragma unroll
@@ -448,6 +491,15 @@ inline int delta_go(const reax::DeltaArgs& a, cudaStream_t st) {
   }
   static SmemAttr attr;
   if (ensure_smem(attr, reax::delta_chunk_kernel, (int)sizeof(reax::DcSmem), true) != cudaSuccess) return -4;
+  // setmaxnreg's shares (four warps of 168 registers a thread, four of 88) come out of the registers of the launch: with fewer
+  // than 128 a thread the kernel would wait for the rest for good
+  static std::atomic<int> regs{0};
+  if (!regs) {
+    cudaFuncAttributes at;
+    if (cudaFuncGetAttributes(&at, reax::delta_chunk_kernel) != cudaSuccess) return -4;
+    regs = at.numRegs;
+  }
+  if (regs < 128) return -4;
   reax::delta_chunk_kernel<<<grid, reax::DC_THREADS, sizeof(reax::DcSmem), st>>>(a);
   reax::delta_step_kernel<<<grid, reax::DS_THREADS, 0, st>>>(a, reax::DS_MOST);
   return (int)cudaGetLastError();
