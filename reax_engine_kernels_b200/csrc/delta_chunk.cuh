@@ -43,7 +43,9 @@ struct DcSmem {
     float frac[DC_T], beta[DC_T];
     float grow[DC_T], left[DC_T];  // 2^G_i, 2^(G_last - G_i)
   } G[3];                          // chunk c's in c % 3
-  float L[DC_T][DC_T + 4];  // column by column; then the inverse, row by row
+  float L[DC_T][DC_T + 4];  // -(strictly lower part) column by column
+  float X[DC_T][DC_T + 4];  // (1 + it)^-1 row by row (only blocks on and below the diagonal)
+  float Y[16][20];
   uint8_t o[4][DC_T * 48];  // per warp: 32 tokens x 16 rows
 };
 
@@ -136,7 +138,7 @@ __device__ __forceinline__ void dc_decays(DcSmem& s, int slot, int lane, float g
 }
 
 // A third of both Gram matrices: w = 0 rows 0-15 by columns 0-15, 1 rows 16-31 by columns 0-15, 2 rows 16-31 by columns 16-31.
-// L = -(strictly lower beta_i 2^(G_i - G_j) k_i . k_j) to s.L, P = lower 2^(G_i - G_j) q_i . k_j in two terms.
+// s.L = -(strictly lower beta_i 2^(G_i - G_j) k_i . k_j), P = lower 2^(G_i - G_j) q_i . k_j in two terms.
 __device__ __forceinline__ void dc_gram(DcSmem& s, const DcIn& in, int slot, DcPrep& out, int w, int lane) {
   const int gq = lane >> 2, t = lane & 3, i0 = w ? 16 : 0, j0 = w == 2 ? 16 : 0;
   const uint32_t ka = smem_u32(in.k), qa = smem_u32(in.q);
@@ -191,25 +193,65 @@ __device__ __forceinline__ void dc_gram(DcSmem& s, const DcIn& in, int slot, DcP
     }
 }
 
-// One warp: column `lane` of (1 + L)^-1 by forward substitution, right-looking: once x_j is final, it leaves the later ones.  Over
-// s.L, row by row.
-__device__ __forceinline__ void dc_inverse(DcSmem& s, int lane) {
-  float x[DC_T];
+// X = (1 - N)^-1 for N = s.L, in fp32, by the four preparing warps.  The 8 x 8 blocks on the diagonal by forward substitution, a
+// column to a lane; then twice [[A, 0], [C, B]]^-1 = [[A', 0], [B' C A', B']] of inverses A', B', first to 16 x 16, then to 32 x 32.
+// One warp's substitution over all 32 rows is a chain of 31 steps with 496 multiply-adds a lane, 4300 cycles at 88 registers.
+__device__ __forceinline__ void dc_inverse(DcSmem& s, int pt) {
+  if (pt < 32) {
+    const int b = pt & 24, col = pt & 7;
+    float l[7][8], x[8];
 #pragma unroll
-  for (int i = 0; i < DC_T; ++i) x[i] = i == lane ? 1.f : 0.f;
+    for (int j = 0; j < 7; ++j)
 #pragma unroll
-  for (int j = 0; j < DC_T - 1; ++j)
+      for (int i = 0; i < 8; i += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(&s.L[b + j][b + i]);
+        l[j][i] = v.x, l[j][i + 1] = v.y, l[j][i + 2] = v.z, l[j][i + 3] = v.w;
+      }
 #pragma unroll
-    for (int i = (j + 1) & ~3; i < DC_T; i += 4) {
-      const float4 l = *reinterpret_cast<const float4*>(&s.L[j][i]);  // what lies on and above the diagonal is not used
-      if (i > j) x[i] = __fmaf_rn(l.x, x[j], x[i]);
-      if (i + 1 > j) x[i + 1] = __fmaf_rn(l.y, x[j], x[i + 1]);
-      if (i + 2 > j) x[i + 2] = __fmaf_rn(l.z, x[j], x[i + 2]);
-      x[i + 3] = __fmaf_rn(l.w, x[j], x[i + 3]);
+    for (int i = 0; i < 8; ++i) x[i] = i == col ? 1.f : 0.f;
+#pragma unroll
+    for (int j = 0; j < 7; ++j)
+#pragma unroll
+      for (int i = j + 1; i < 8; ++i) x[i] = __fmaf_rn(l[j][i], x[j], x[i]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s.X[b + i][b + col] = x[i];
+  }
+  named_bar_sync<1, 128>();
+  {
+    const int j0 = pt >> 6 << 4, i0 = j0 + 8, r = (pt >> 3) & 7, c = pt & 7;
+    float y = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) y = __fmaf_rn(s.L[j0 + k][i0 + r], s.X[j0 + k][j0 + c], y);
+    s.Y[(pt >> 6 << 3) + r][c] = y;
+    s.X[j0 + r][i0 + c] = 0.f;
+    named_bar_sync<1, 128>();
+    float z = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) z = __fmaf_rn(s.X[i0 + r][i0 + k], s.Y[(pt >> 6 << 3) + k][c], z);
+    s.X[i0 + r][j0 + c] = z;
+  }
+  named_bar_sync<1, 128>();
+  {
+    const int r = pt >> 3, c = (pt & 7) * 2;
+    float y0 = 0.f, y1 = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const float2 x = *reinterpret_cast<const float2*>(&s.X[k][c]);
+      const float n = s.L[k][16 + r];
+      y0 = __fmaf_rn(n, x.x, y0), y1 = __fmaf_rn(n, x.y, y1);
     }
-  __syncwarp();  // every lane has read L
+    *reinterpret_cast<float2*>(&s.Y[r][c]) = make_float2(y0, y1);
+    named_bar_sync<1, 128>();
+    float z0 = 0.f, z1 = 0.f;
 #pragma unroll
-  for (int i = 0; i < DC_T; ++i) s.L[i][lane] = x[i];
+    for (int k = 0; k < 16; ++k) {
+      const float2 y = *reinterpret_cast<const float2*>(&s.Y[k][c]);
+      const float x = s.X[16 + r][16 + k];
+      z0 = __fmaf_rn(x, y.x, z0), z1 = __fmaf_rn(x, y.y, z1);
+    }
+    *reinterpret_cast<float2*>(&s.X[16 + r][c]) = make_float2(z0, z1);
+  }
+  named_bar_sync<1, 128>();
 }
 
 // T = inverse * beta_j in three terms; thread pt of the 128 takes 8 columns of a row
@@ -218,7 +260,7 @@ __device__ __forceinline__ void dc_terms(const DcSmem& s, int slot, DcPrep& out,
   uint32_t y[3][4];
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    const float2 x = *reinterpret_cast<const float2*>(&s.L[i][j + 2 * c]), b = *reinterpret_cast<const float2*>(&s.G[slot].beta[j + 2 * c]);
+    const float2 x = *reinterpret_cast<const float2*>(&s.X[i][j + 2 * c]), b = *reinterpret_cast<const float2*>(&s.G[slot].beta[j + 2 * c]);
     uint32_t z[3];
     split_bf16<3>(x.x * b.x, x.y * b.y, z);
 #pragma unroll
@@ -235,8 +277,7 @@ __device__ __forceinline__ void dc_prepare(DcSmem& s, int c, int w, int lane, De
   DcPrep& out = s.prep[c & 1];
   if (w < 3) dc_gram(s, s.in[c % 3], c % 3, out, w, lane);
   named_bar_sync<1, 128>();
-  if (w == 3) dc_inverse(s, lane);
-  named_bar_sync<1, 128>();
+  dc_inverse(s, w * 32 + lane);
   dc_terms(s, c % 3, out, w * 32 + lane);
   if (w == 3) decays();
 }
