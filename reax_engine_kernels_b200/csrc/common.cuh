@@ -554,6 +554,11 @@ __device__ __forceinline__ void tmem_ld_16x256b_x2(uint32_t taddr, uint32_t (&r)
       : "r"(taddr)
       : "memory");
 }
+// Programmatic dependent launch: the next kernel's CTAs may start once every CTA of this one has come here (or left), and
+// wait for all of this one's results at their pdl_wait.
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // make this thread's generic-proxy shared-memory writes (st.shared, cp.async) visible to the async proxy (tcgen05.mma)
 __device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -656,6 +661,22 @@ inline cudaError_t ensure_smem(SmemAttr& a, K kernel, int bytes, bool max_shared
   if (dev < 0 || dev >= 64) return set();
   std::call_once(a.flags[dev], [&] { a.err[dev] = set(); });
   return a.err[dev];
+}
+
+// One launch; dependent: as a programmatic dependent of the launch before it in the stream (see pdl_launch)
+template <typename... P, typename... A>
+inline int launch_dependent(void (*kernel)(P...), dim3 grid, int threads, int smem, bool dependent, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = dependent ? 1 : 0;
+  return (int)cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
 
 }  // namespace reax_host

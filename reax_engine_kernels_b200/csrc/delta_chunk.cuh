@@ -307,6 +307,7 @@ __device__ __forceinline__ int dc_sequence(const DeltaArgs& a) {
 __global__ void __launch_bounds__(DC_THREADS, 2) delta_chunk_kernel(DeltaArgs a) {
   extern __shared__ __align__(128) uint8_t dc_raw[];
   DcSmem& s = *reinterpret_cast<DcSmem*>(dc_raw);
+  pdl_launch();  // the step kernel's sequences are others
   const int n = dc_sequence(a), hv = blockIdx.y, lane = threadIdx.x & 31, warp = warp_id();
   const int gq = lane >> 2, t4 = lane & 3, row0 = blockIdx.x * 64;
   long long t0, e;
@@ -542,8 +543,8 @@ inline int delta_go(const reax::DeltaArgs& a, cudaStream_t st) {
   }
   if (regs < 128) return -4;
   reax::delta_chunk_kernel<<<grid, reax::DC_THREADS, sizeof(reax::DcSmem), st>>>(a);
-  reax::delta_step_kernel<<<grid, reax::DS_THREADS, 0, st>>>(a, reax::DS_MOST);
-  return (int)cudaGetLastError();
+  if (cudaError_t e = cudaGetLastError()) return (int)e;
+  return launch_dependent(reax::delta_step_kernel, grid, reax::DS_THREADS, 0, true, st, a, reax::DS_MOST);
 }
 
 }  // namespace reax_host

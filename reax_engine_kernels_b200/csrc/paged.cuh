@@ -103,10 +103,6 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
 __device__ __forceinline__ void cp_async16_full(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-// Programmatic dependent launch: the next kernel's CTAs may start once every CTA of this one has come here (or left), and
-// wait for all of this one's results at their pdl_wait.
-__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // A maximum for use as a subtrahend: -inf replaced
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
 

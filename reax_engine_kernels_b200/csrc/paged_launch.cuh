@@ -48,22 +48,6 @@ inline int paged_check(int B, int H, int M, int G, int D, int P, int page, int L
   return 0;
 }
 
-// One launch of 128 threads a CTA; dependent: as a programmatic dependent of the launch before it
-inline int launch_dependent(void (*kernel)(const reax::PagedArgs), dim3 grid, int smem, bool dependent, const reax::PagedArgs& a,
-                            cudaStream_t st) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(128);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = dependent ? 1 : 0;
-  return (int)cudaLaunchKernelEx(&cfg, kernel, a);
-}
-
 template <int D, int RT, bool PRE>
 inline int paged_launch(const reax::PagedArgs& a, cudaStream_t st) {
   using C = reax::PagedCfg<D, RT>;
@@ -71,7 +55,7 @@ inline int paged_launch(const reax::PagedArgs& a, cudaStream_t st) {
   if (ensure_smem(attr, reax::paged_kernel<D, RT, PRE>, C::SMEM, true) != cudaSuccess) return -4;
   const long long x = PRE ? (long long)ceil_div((long long)a.B * a.M, C::ROWS) * a.psplits : (long long)ceil_div(a.M, C::ROWS) * a.splits;
   if (x > 0x7fffffffLL) return -1;
-  return launch_dependent(reax::paged_kernel<D, RT, PRE>, dim3((unsigned)x, a.H, PRE ? 1 : a.B), C::SMEM, !PRE && a.psplits, a, st);
+  return launch_dependent(reax::paged_kernel<D, RT, PRE>, dim3((unsigned)x, a.H, PRE ? 1 : a.B), 128, C::SMEM, !PRE && a.psplits, st, a);
 }
 
 template <int D>
@@ -93,7 +77,7 @@ inline int paged_go(const reax::PagedArgs& a, cudaStream_t st) {
   if (int rc = a.M <= 8 ? paged_launch<D, 1, false>(a, st) : paged_launch<D, 2, false>(a, st)) return rc;
   if (a.splits + a.psplits > 1) {
     const dim3 rows((unsigned)((long long)a.B * a.H * a.M));
-    return launch_dependent(a.M <= 8 ? reax::paged_join_kernel<D, 8> : reax::paged_join_kernel<D, 16>, rows, 0, true, a, st);
+    return launch_dependent(a.M <= 8 ? reax::paged_join_kernel<D, 8> : reax::paged_join_kernel<D, 16>, rows, 128, 0, true, st, a);
   }
   return 0;
 }
