@@ -663,19 +663,29 @@ inline cudaError_t ensure_smem(SmemAttr& a, K kernel, int bytes, bool max_shared
   return a.err[dev];
 }
 
-// One launch; dependent: as a programmatic dependent of the launch before it in the stream (see pdl_launch)
+// One launch; dependent: as a programmatic dependent of the launch before it in the stream (see pdl_launch); cluster: CTAs per
+// cluster, along x
 template <typename... P, typename... A>
-inline int launch_dependent(void (*kernel)(P...), dim3 grid, int threads, int smem, bool dependent, cudaStream_t st, A... args) {
+inline int launch_dependent(void (*kernel)(P...), dim3 grid, int threads, int smem, bool dependent, cudaStream_t st, int cluster, A... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = dependent ? 1 : 0;
+  cudaLaunchAttribute attr[2]{};
+  int n = 0;
+  if (dependent) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
   return (int)cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
 

@@ -7,5 +7,4 @@
 
 REAX_DEFINE_STATUS_EXPORT()
 REAX_DEFINE_KV_EXPORTS()
-REAX_DEFINE_PAGED_EXPORTS()
 REAX_DEFINE_DELTA_STATE_EXPORT()

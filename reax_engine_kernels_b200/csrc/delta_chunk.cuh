@@ -544,7 +544,7 @@ inline int delta_go(const reax::DeltaArgs& a, cudaStream_t st) {
   if (regs < 128) return -4;
   reax::delta_chunk_kernel<<<grid, reax::DC_THREADS, sizeof(reax::DcSmem), st>>>(a);
   if (cudaError_t e = cudaGetLastError()) return (int)e;
-  return launch_dependent(reax::delta_step_kernel, grid, reax::DS_THREADS, 0, true, st, a, reax::DS_MOST);
+  return launch_dependent(reax::delta_step_kernel, grid, reax::DS_THREADS, 0, true, st, 1, a, reax::DS_MOST);
 }
 
 }  // namespace reax_host

@@ -9,7 +9,8 @@
 // HBM-bound: every visible cache byte is read once per key/value head, for all of the head's rows together.  A CTA of four warps
 // takes 8 or 16 rows of one (sequence, head) and a chunk of its keys; each warp takes every fourth group of 16 keys, streams them
 // through its own cp.async ring (no barrier in the loop) and keeps its own sums; the four are merged through shared memory,
-// the chunks by paged_join_kernel.  A sequence that fits one chunk is written by its only CTA.
+// up to eight chunks of a sequence through the distributed shared memory of their cluster, more (or a prefix) by
+// paged_join_kernel.
 //
 // The products are transposed, S^T = K Q^T and O^T = V^T P^T, so that keys and value columns fill the 16 rows of an m16n8k16 and
 // the 4 to 8 query rows of a decode step its 8 columns.  With query rows as the 16 (the first version of this kernel, 3.5 TB/s over
@@ -53,8 +54,9 @@ struct PagedArgs {
   const int* prefix;  // page ids of the shared prefix, NULL without one
   float scale_log2;
   int B, H, M, G, P, page, shift, Lp;
-  int chunk, splits;    // the sequences' own keys: keys per chunk, chunks
-  int pchunk, psplits;  // the same of the prefix
+  int chunk, splits;    // a sequence's own keys: keys per chunk, chunks
+  int cluster;          // 1: the CTAs of one tile's chunks are a cluster and join their results themselves
+  int pchunk, psplits;  // the prefix: keys per chunk, chunks
   long long pages;
 };
 
@@ -118,6 +120,22 @@ __device__ __forceinline__ int paged_visible(const PagedArgs& a, int b, int r0, 
   return min(max(lim, -1), a.P * a.page - 1) + 1;
 }
 
+// Keys per chunk of a tile that sees n: fixed, or for a cluster even shares of 64 keys (16 for each warp) or more
+__device__ __forceinline__ int paged_chunk(const PagedArgs& a, int n) {
+  return a.cluster ? max(((n + a.splits - 1) / a.splits + 63) & ~63, 64) : a.chunk;
+}
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float x;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(addr) : "memory");
+  return x;
+}
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
+  float4 x;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(addr) : "memory");
+  return x;
+}
+
 // q rows as f16 in shared memory, each scaled by a power of two; srow[r] takes it out again.  128 threads, 8 per row.
 template <int D, int ROWS, int QP, typename RowPtr>
 __device__ __forceinline__ void paged_load_q(char* sq, float* srow, RowPtr row_ptr, float scale_log2) {
@@ -160,7 +178,8 @@ __global__ void __launch_bounds__(128, PagedCfg<D, RT>::CTAS) paged_kernel(const
   extern __shared__ __align__(128) char smem[];
   __shared__ float srow[ROWS];
   __shared__ float sm[C::WARPS][3][ROWS];
-  const int nsplit = PRE ? a.psplits : a.splits, chunk = PRE ? a.pchunk : a.chunk;
+  __shared__ float slse[ROWS];
+  const int nsplit = PRE ? a.psplits : a.splits;
   const int h = blockIdx.y, split = blockIdx.x % nsplit, r0 = blockIdx.x / nsplit * ROWS;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   // batch entry and row of the CTA's row i; r >= M: there is none
@@ -170,9 +189,11 @@ __global__ void __launch_bounds__(128, PagedCfg<D, RT>::CTAS) paged_kernel(const
     if (PRE && b >= a.B) b = 0, r = a.M;
   };
   const int n = PRE ? a.Lp : paged_visible<ROWS>(a, blockIdx.z, r0, lane);
-  const int c0 = split * chunk, c1 = min(n, c0 + chunk);
-  const bool direct = !PRE && a.psplits == 0 && n <= chunk;  // the only chunk writes the output itself
-  if (c0 >= n && !(direct && split == 0)) {
+  const int chunk = PRE ? a.pchunk : paged_chunk(a, n);
+  const int c0 = min(split * chunk, n), c1 = min(n, c0 + chunk);
+  const bool cluster = !PRE && a.cluster;
+  const bool direct = !PRE && !cluster && a.psplits == 0 && n <= chunk;  // the only chunk writes the output itself
+  if (c0 >= n && !(direct && split == 0) && !cluster) {
     if (!PRE) pdl_wait();
     return;
   }
@@ -445,39 +466,75 @@ __global__ void __launch_bounds__(128, PagedCfg<D, RT>::CTAS) paged_kernel(const
   // behind it finds both results
   if (!PRE) pdl_wait();
   const int row = threadIdx.x >> 3, sub = threadIdx.x & 7;  // 8 threads a row
-  if (row >= ROWS) return;
-  int b, mr;
-  row_of(row, b, mr);
-  if (mr >= a.M) return;
-  float top = -INFINITY, topv = -INFINITY, sum = 0.f;
+  const long long rows = (long long)a.B * a.H * a.M;
+  if (row < ROWS) {
+    int b, mr;
+    row_of(row, b, mr);
+    float top = -INFINITY, topv = -INFINITY, sum = 0.f;
 #pragma unroll
-  for (int w = 0; w < C::WARPS; ++w) top = fmaxf(top, sm[w][0][row]), topv = fmaxf(topv, sm[w][1][row]);
+    for (int w = 0; w < C::WARPS; ++w) top = fmaxf(top, sm[w][0][row]), topv = fmaxf(topv, sm[w][1][row]);
 #pragma unroll
-  for (int w = 0; w < C::WARPS; ++w) sum += sm[w][2][row] * ex2_approx(sm[w][0][row] - finite_or_zero(top));
-  const float fac = sum == 0.f ? 0.f : ex2_approx(finite_or_zero(topv) - finite_or_zero(top)) / sum;
-  const long long R = ((long long)b * a.H + h) * a.M + mr, rows = (long long)a.B * a.H * a.M;
-  const long long at = (PRE ? a.splits + split : split) * rows + R;
+    for (int w = 0; w < C::WARPS; ++w) sum += sm[w][2][row] * ex2_approx(sm[w][0][row] - finite_or_zero(top));
+    const float fac = sum == 0.f ? 0.f : ex2_approx(finite_or_zero(topv) - finite_or_zero(top)) / sum;
+    const float lse = sum == 0.f ? -INFINITY : top + log2f(sum);
+    const long long at = (PRE ? a.splits + split : split) * rows + ((long long)b * a.H + h) * a.M + mr;
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) {
-    const int d = (i * 8 + sub) * 8;
-    float v[8];
+    for (int i = 0; i < D / 64; ++i) {
+      const int d = (i * 8 + sub) * 8;
+      float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      v[e] = 0.f;
+      for (int e = 0; e < 8; ++e) {
+        v[e] = 0.f;
 #pragma unroll
-      for (int w = 0; w < C::WARPS; ++w) v[e] += so[(w * ROWS + row) * C::OP + d + e];
-      v[e] = sum == 0.f ? 0.f : v[e] * fac;
+        for (int w = 0; w < C::WARPS; ++w) v[e] += so[(w * ROWS + row) * C::OP + d + e];
+        v[e] = sum == 0.f ? 0.f : v[e] * fac;
+      }
+      if (direct && mr < a.M)
+        *reinterpret_cast<uint4*>(a.o + b * a.oB + h * a.oH + mr * a.oM + d) =
+            make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+      if (!direct && (cluster || mr < a.M)) {  // for the cluster in this CTA's shared memory, over the first warp's share
+        float4* p = reinterpret_cast<float4*>(cluster ? so + row * C::OP + d : a.part + at * D + d);
+        p[0] = make_float4(v[0], v[1], v[2], v[3]);
+        p[1] = make_float4(v[4], v[5], v[6], v[7]);
+      }
     }
-    if (direct) {
-      *reinterpret_cast<uint4*>(a.o + b * a.oB + h * a.oH + mr * a.oM + d) =
-          make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
-    } else {
-      float4* p = reinterpret_cast<float4*>(a.part + at * D + d);
-      p[0] = make_float4(v[0], v[1], v[2], v[3]);
-      p[1] = make_float4(v[4], v[5], v[6], v[7]);
+    if (sub == 0) {
+      if (cluster) slse[row] = lse;
+      else if (!direct && mr < a.M) a.lse[at] = lse;
     }
   }
-  if (!direct && sub == 0) a.lse[at] = sum == 0.f ? -INFINITY : top + log2f(sum);
+  if (!cluster) return;
+
+  // ---- join the cluster's chunks, four values of a row per thread
+  cluster_sync_all();
+  const uint32_t so_u = smem_u32(so), lse_u = smem_u32(slse);
+  for (int x = split * 128 + threadIdx.x; x < ROWS * (D / 4); x += nsplit * 128) {
+    const int r = x / (D / 4), d = x % (D / 4) * 4;
+    int b, mr;
+    row_of(r, b, mr);
+    if (mr >= a.M) continue;
+    float w[8], top = -INFINITY, sum = 0.f;
+    float4 p[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < nsplit) {
+        w[i] = ld_cluster_f32(mapa_shared(lse_u + r * 4, i));
+        p[i] = ld_cluster_v4(mapa_shared(so_u + (r * C::OP + d) * 4, i));
+        top = fmaxf(top, w[i]);
+      }
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < nsplit) {
+        const float f = ex2_approx(w[i] - finite_or_zero(top));  // a NaN stays one
+        sum += f;
+        acc.x += f * p[i].x, acc.y += f * p[i].y, acc.z += f * p[i].z, acc.w += f * p[i].w;
+      }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    *reinterpret_cast<uint2*>(a.o + b * a.oB + h * a.oH + mr * a.oM + d) =
+        make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+  }
+  cluster_sync_all();  // no CTA leaves while another reads its shared memory
 }
 
 // Joins the chunks' partial outputs: one CTA per row; D / 4 threads take four values each, 128 / (D / 4) groups of them every other
@@ -492,8 +549,8 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
   const int r = (int)(R % a.M), h = (int)(R / a.M % a.H), b = (int)(R / a.M / a.H);
   const int n = paged_visible<ROWS>(a, b, r & ~(ROWS - 1), lane);
   pdl_wait();
-  if (a.psplits == 0 && n <= a.chunk) return;  // written by its only chunk
-  const int mine = (n + a.chunk - 1) / a.chunk, total = mine + a.psplits;
+  const int chunk = paged_chunk(a, n), mine = (n + chunk - 1) / chunk, total = mine + a.psplits;
+  if (a.psplits == 0 && n <= chunk) return;  // written by its only chunk
   auto slot = [&](int i) { return (i < mine ? i : a.splits + i - mine) * rows + R; };
   float top = -INFINITY;
   bool nan = false;

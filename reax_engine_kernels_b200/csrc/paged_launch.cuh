@@ -6,36 +6,48 @@
 namespace reax_host {
 
 struct PagedPlan {
-  int chunk, splits, pchunk, psplits;
+  int chunk, splits, cluster, pchunk, psplits;
 };
 inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
 // Whether the prefix goes to prefix_kernel (128 rows a CTA): from the second group of 16 rows on paged_kernel would read it twice.
 inline bool prefix_tiled(int B, int M) { return (long long)B * M > 16; }
 
-// Chunks of the keys, from the shapes alone (the lengths are on the device, and a captured launch replays with others): as
-// many CTAs as keep every SM at its resident count about three times over when all sequences are full, but no chunk under 256
-// keys, 64 for each of the four warps.
+// Chunks of the keys, from the shapes alone (the lengths are on the device, and a captured launch replays with others).
+//  * Few CTAs: as many chunks, up to the 8 of a cluster, as fit the GPU twice over with 64 keys (16 for each warp) or more in
+//    each, joined within the cluster; as long as a chunk then is no longer than 256 keys.  One sequence of 1024 keys (8 heads of
+//    128): 6.4 us, against 8.6 with the join in a kernel of its own and 15.5 in one chunk; of 4096, where a chunk would be
+//    512: 11.0 against 9.9.
+//  * Otherwise fixed chunks, as many CTAs as make three waves when all sequences are full: short sequences then leave at once, and
+//    long ones spread.  Even shares take 37 us where these take 25 (32 ragged sequences up to 2048 keys).  No chunk under 256
+//    keys; none under 1024 where the sequences alone fill half the GPU (64 of up to 1024 keys: 26 -> 23 us); no more than 32
+//    chunks once they are two CTAs an SM (one sequence of 65536 keys: 57 us in 205 chunks, 38 in 32).
 inline PagedPlan paged_plan(int B, int H, int M, int D, int P, int page, int Lp, int sms) {
   auto cut = [&](long long keys, long long units, int resident, int& chunk, int& splits) {
-    const long long want = (3LL * sms * resident + units - 1) / units;
-    long long c = (keys + want - 1) / want;
-    c = (c + 63) / 64 * 64;
-    chunk = (int)(c < 256 ? 256 : c);
+    const long long slots = (long long)sms * resident, floor = 2 * units > slots ? 1024 : 256;
+    const long long most = 2LL * sms > 32 * units ? (2LL * sms + units - 1) / units : 32;
+    const long long three = (3 * slots + units - 1) / units, want = three < most ? three : most;
+    const long long c = ((keys + want - 1) / want + 63) / 64 * 64;
+    chunk = (int)(c < floor ? floor : c);
     splits = keys ? ceil_div(keys, chunk) : 0;
   };
   const int rows = M <= 8 ? 8 : 16, resident = M <= 8 ? (D == 256 ? 3 : 4) : (D == 256 ? 2 : 3);
+  const long long keys = (long long)P * page, units = (long long)B * H * ceil_div(M, rows);
   PagedPlan p;
-  cut((long long)P * page, (long long)B * H * ceil_div(M, rows), resident, p.chunk, p.splits);
+  cut(keys, units, resident, p.chunk, p.splits);
+  if (p.splits == 0) p.splits = 1;  // no pages at all: one chunk without keys
+  int s = 1;
+  while (s < 8 && 2 * s * units <= 2LL * sms && keys >= 2 * s * 64) s *= 2;
+  p.cluster = Lp == 0 && s > 1 && keys <= 256LL * s;
+  if (p.cluster) p.splits = s;
   if (prefix_tiled(B, M)) {  // one CTA of 128 rows per SM; two tiles of 64 keys at least
-    const long long units = (long long)H * ceil_div((long long)B * M, reax::PF_ROWS), want = units < sms ? sms / units : 1;
+    const long long tiles = (long long)H * ceil_div((long long)B * M, reax::PF_ROWS), want = tiles < sms ? sms / tiles : 1;
     const int c = ceil_div(ceil_div(Lp, want), reax::PF_BN) * reax::PF_BN;
     p.pchunk = c < 2 * reax::PF_BN ? 2 * reax::PF_BN : c;
     p.psplits = ceil_div(Lp, p.pchunk);
   } else {
     cut(Lp, (long long)H * ceil_div((long long)B * M, 16), D == 256 ? 2 : 3, p.pchunk, p.psplits);
   }
-  if (p.splits == 0) p.splits = 1;  // no pages at all: one chunk without keys
   return p;
 }
 
@@ -55,7 +67,8 @@ inline int paged_launch(const reax::PagedArgs& a, cudaStream_t st) {
   if (ensure_smem(attr, reax::paged_kernel<D, RT, PRE>, C::SMEM, true) != cudaSuccess) return -4;
   const long long x = PRE ? (long long)ceil_div((long long)a.B * a.M, C::ROWS) * a.psplits : (long long)ceil_div(a.M, C::ROWS) * a.splits;
   if (x > 0x7fffffffLL) return -1;
-  return launch_dependent(reax::paged_kernel<D, RT, PRE>, dim3((unsigned)x, a.H, PRE ? 1 : a.B), 128, C::SMEM, !PRE && a.psplits, st, a);
+  const dim3 grid((unsigned)x, a.H, PRE ? 1 : a.B);
+  return launch_dependent(reax::paged_kernel<D, RT, PRE>, grid, 128, C::SMEM, !PRE && a.psplits, st, !PRE && a.cluster ? a.splits : 1, a);
 }
 
 template <int D>
@@ -75,13 +88,58 @@ inline int paged_go(const reax::PagedArgs& a, cudaStream_t st) {
   if (a.psplits)
     if (int rc = prefix_tiled(a.B, a.M) ? prefix_launch<D>(a, st) : paged_launch<D, 2, true>(a, st)) return rc;
   if (int rc = a.M <= 8 ? paged_launch<D, 1, false>(a, st) : paged_launch<D, 2, false>(a, st)) return rc;
-  if (a.splits + a.psplits > 1) {
+  if (a.splits + a.psplits > 1 && !a.cluster) {
     const dim3 rows((unsigned)((long long)a.B * a.H * a.M));
-    return launch_dependent(a.M <= 8 ? reax::paged_join_kernel<D, 8> : reax::paged_join_kernel<D, 16>, rows, 128, 0, true, st, a);
+    return launch_dependent(a.M <= 8 ? reax::paged_join_kernel<D, 8> : reax::paged_join_kernel<D, 16>, rows, 128, 0, true, st, 1, a);
   }
   return 0;
 }
 
 }  // namespace reax_host
 
-#define REAX_DEFINE_PAGED_EXPORTS()                                                                                      REAX_API int reax_fmha_paged_splits(int B, int H, int M, int D, int P, int page, int Lp) {                                  if (int rc = reax_host::paged_check(B, H, M, 1, D, P, page, Lp)) return rc;                                              int dev = 0;                                                                                                             if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;                                                                         const reax_host::PagedPlan p = reax_host::paged_plan(B > 0 ? B : 1, H, M > 0 ? M : 1, D, P, page, Lp,                                                                         reax_host::device_sms(dev));                                        return p.splits + p.psplits;                                                                                           }                                                                                                                        REAX_API int reax_fmha_paged(const void* q, long long qsB, long long qsH, long long qsM, const void* kc, const void* ke,                                const void* vc, const void* ve, long long csP, long long csH, long long esP,                                             long long esH, const int* table, long long tsB, const int* prefix, int prefix_len,                                       const int* qpos, int G, long long qpBs, void* o, long long osB, long long osH,                                           long long osM, void* ws, float scale, int B, int H, int M, int D, int P, int page,                                       long long pages, void* stream) {                                                              const int Lp = prefix_len;                                                                                               if (int rc = reax_host::paged_check(B, H, M, G, D, P, page, Lp)) return rc;                                              if (B == 0 || M == 0) return 0;                                                                                          if (!q || !qpos || !o || pages < 0 || (P > 0 && !table) || (Lp > 0 && !prefix)) return -1;                                if ((P > 0 || Lp > 0) && (!kc || !ke || !vc || !ve)) return -1;                                                           if (((uintptr_t)q | (uintptr_t)o | (uintptr_t)kc | (uintptr_t)vc | (uintptr_t)ke | (uintptr_t)ve | (uintptr_t)ws) & 15)       return -1;                                                                                                             if ((qsB | qsH | qsM | osB | osH | osM) & 7) return -1;                                                                  if ((csP | csH | esP | esH) & 15) return -1;                                                                             int dev = 0;                                                                                                             cudaGetDevice(&dev);                                                                                                     const reax_host::PagedPlan p = reax_host::paged_plan(B, H, M, D, P, page, Lp, reax_host::device_sms(dev));               const int splits = p.splits + p.psplits;                                                                                 if (splits > 1 && !ws) return -5;                                                                                        float* part = (float*)ws;                                                                                                reax::PagedArgs a{(const uint16_t*)q, qsB, qsH, qsM, (const uint8_t*)kc, (const uint8_t*)ke, (const uint8_t*)vc,                             (const uint8_t*)ve, csP, csH, esP, esH, table, tsB, qpos, qpBs, (uint16_t*)o, osB, osH, osM, part,                         part ? part + (long long)splits * B * H * M * D : nullptr, Lp ? prefix : nullptr,                                        scale * 1.4426950408889634f, B, H, M, G, P, page, reax_host::page_shift(page), Lp, p.chunk,                              p.splits, p.pchunk, p.psplits, pages};                                                                 return D == 128 ? reax_host::paged_go<128>(a, (cudaStream_t)stream) : reax_host::paged_go<256>(a, (cudaStream_t)stream);   }
+// ------------------------------------------------------------------------------------------------
+// exported entry points
+// ------------------------------------------------------------------------------------------------
+REAX_API int reax_fmha_paged_splits(int B, int H, int M, int D, int P, int page, int Lp) {
+  if (int rc = reax_host::paged_check(B, H, M, 1, D, P, page, Lp)) return rc;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
+  const reax_host::PagedPlan p =
+      reax_host::paged_plan(B > 0 ? B : 1, H, M > 0 ? M : 1, D, P, page, Lp, reax_host::device_sms(dev));
+  return p.cluster ? 1 : p.splits + p.psplits;
+}
+
+REAX_API int reax_fmha_paged(const void* q, long long qsB, long long qsH, long long qsM, const void* kc, const void* ke,
+                             const void* vc, const void* ve, long long csP, long long csH, long long esP, long long esH,
+                             const int* table, long long tsB, const int* prefix, int prefix_len, const int* qpos, int G,
+                             long long qpBs, void* o, long long osB, long long osH, long long osM, void* ws, float scale,
+                             int B, int H, int M, int D, int P, int page, long long pages, void* stream) {
+  const int Lp = prefix_len;
+  if (int rc = reax_host::paged_check(B, H, M, G, D, P, page, Lp)) return rc;
+  if (B == 0 || M == 0) return 0;
+  if (!q || !qpos || !o || pages < 0 || (P > 0 && !table) || (Lp > 0 && !prefix)) return -1;
+  if ((P > 0 || Lp > 0) && (!kc || !ke || !vc || !ve)) return -1;
+  if (((uintptr_t)q | (uintptr_t)o | (uintptr_t)kc | (uintptr_t)vc | (uintptr_t)ke | (uintptr_t)ve | (uintptr_t)ws) & 15)
+    return -1;
+  if ((qsB | qsH | qsM | osB | osH | osM) & 7) return -1;
+  if ((csP | csH | esP | esH) & 15) return -1;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const reax_host::PagedPlan p = reax_host::paged_plan(B, H, M, D, P, page, Lp, reax_host::device_sms(dev));
+  const int splits = p.cluster ? 1 : p.splits + p.psplits;  // partial results in the workspace
+  if (splits > 1 && !ws) return -5;
+  float* part = (float*)ws;
+  reax::PagedArgs a{};
+  a.q = (const uint16_t*)q, a.qB = qsB, a.qH = qsH, a.qM = qsM;
+  a.kc = (const uint8_t*)kc, a.ke = (const uint8_t*)ke, a.vc = (const uint8_t*)vc, a.ve = (const uint8_t*)ve;
+  a.cP = csP, a.cH = csH, a.eP = esP, a.eH = esH;
+  a.table = table, a.tB = tsB, a.qpos = qpos, a.qpB = qpBs;
+  a.o = (uint16_t*)o, a.oB = osB, a.oH = osH, a.oM = osM;
+  a.part = part, a.lse = part ? part + (long long)splits * B * H * M * D : nullptr;
+  a.prefix = Lp ? prefix : nullptr;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.B = B, a.H = H, a.M = M, a.G = G, a.P = P, a.page = page, a.shift = reax_host::page_shift(page), a.Lp = Lp;
+  a.chunk = p.chunk, a.splits = p.splits, a.cluster = p.cluster, a.pchunk = p.pchunk, a.psplits = p.psplits;
+  a.pages = pages;
+  return D == 128 ? reax_host::paged_go<128>(a, (cudaStream_t)stream) : reax_host::paged_go<256>(a, (cudaStream_t)stream);
+}
