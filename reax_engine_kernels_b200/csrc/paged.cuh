@@ -22,10 +22,11 @@
 // stream needs 180 of the 1024 multiply-adds per clock per SM that it sustains.
 //
 // The value row's power of two cannot be applied after the product, and p * 2^nv may leave f16's range, so p's partner
-// carries it: with x_j the score in the log2 domain, P_j = 2^(x_j + nv_j - m'), feeds the product, while the sum takes 2^(x_j - m);
-// the two references meet in one factor 2^(m' - m) at the end.  m and m' follow the maxima of x and x + nv lazily: they are
-// raised to the maximum only when a score passes them by more than 8 (P <= 2^8 is well within f16, and 2^-14 of the largest
-// weight still is a normal number), which one vote per 16 keys finds out.
+// carries it: with x_j the score in the log2 domain and p_j = 2^(x_j - m), P_j = p_j * 2^nv_j * 2^(m - m') feeds the product, while the
+// sum takes p_j; the two references meet in one factor 2^(m' - m) at the end.  m and m' follow the maxima of x and x + nv lazily:
+// they are raised to the maximum only when a p or P passes 2^8 (well within f16, and 2^-14 of the largest weight still is a
+// normal number), which one vote per 16 keys finds out.  With both exponents taken for each score, and both references
+// compared with it, a group of 16 keys took 373 instructions a warp at D = 128, a third of them for 4 scores a thread.
 //
 // Fragments without shuffles: the k index of q . k may be permuted as long as q and k agree, so a thread takes 16 adjacent
 // bytes of a key row (four k16 steps at once).  ldmatrix.m16n16.trans.b8 leaves four consecutive keys of a value column in a register,
@@ -105,6 +106,8 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
 __device__ __forceinline__ void cp_async16_full(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+// The reference of a row that has seen no key yet: anything passes it, and it weighs nothing beside a real one
+constexpr float PAGED_NONE = -1e30f;
 // A maximum for use as a subtrahend: -inf replaced
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
 
@@ -288,7 +291,7 @@ __global__ void __launch_bounds__(128, PagedCfg<D, RT>::CTAS) paged_kernel(const
   }
 
   float o[RT][D / 16][4];
-  float m[RT][2], mv[RT][2], l[RT][2];
+  float m[RT][2], mv[RT][2], rho[RT][2], l[RT][2];  // rho = 2^(m - mv)
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
@@ -296,7 +299,7 @@ __global__ void __launch_bounds__(128, PagedCfg<D, RT>::CTAS) paged_kernel(const
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[rt][j][e] = 0.f;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) m[rt][e] = mv[rt][e] = -INFINITY, l[rt][e] = 0.f;
+    for (int e = 0; e < 2; ++e) m[rt][e] = mv[rt][e] = PAGED_NONE, rho[rt][e] = 1.f, l[rt][e] = 0.f;
   }
   const int key = 4 * (g >> 1) + (g & 1);  // this thread's keys: key and key + 2
   // A row's chunk c ^ swz: the part of c that the unrolled loops count stays out of the XOR
@@ -311,6 +314,7 @@ __global__ void __launch_bounds__(128, PagedCfg<D, RT>::CTAS) paged_kernel(const
     __syncwarp();
     const int j0 = c0 + (warp + C::WARPS * i) * 16;
     const char* st = ring + slot * C::STAGE;
+    const bool ok = *reinterpret_cast<const int*>(st + 2 * C::TILE + 32);
     const char *kr0 = st + key * D + ksw, *kr1 = st + (key + 2) * D + ksw2;
     const uint32_t vr = ring_u + slot * C::STAGE + C::TILE + vrow * D;
     slot = slot + 1 == C::STAGES ? 0 : slot + 1;
@@ -337,50 +341,59 @@ __global__ void __launch_bounds__(128, PagedCfg<D, RT>::CTAS) paged_kernel(const
         }
       }
     }
-    // ---- scale, mask
+    // ---- weights; the exponent bytes of the thread's two keys (255, a NaN row, becomes an infinity)
     const char* meta = st + 2 * C::TILE;
-    const float ks[2] = {pow2_byte((uint8_t)meta[key]), pow2_byte((uint8_t)meta[key + 2])};
-    float nv[2];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int vbyte = (uint8_t)meta[16 + key + 2 * r];
-      nv[r] = vbyte == 255 ? __uint_as_float(0x7fc00000u) : (float)(vbyte - 127);
-    }
-    float x[RT][2][2], y[RT][2][2];  // [key][row]
-    bool over = false;
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) x[rt][r][e] = (s[rt][0][2 * r + e] + s[rt][1][2 * r + e]) * (rs[rt][e] * ks[r]);
-    if (__any_sync(0xffffffffu, j0 + 15 > least) || !*reinterpret_cast<const int*>(meta + 32)) {
-      const bool ok = *reinterpret_cast<const int*>(meta + 32);
+    const uint32_t kx = *reinterpret_cast<const uint32_t*>(meta + (key & 12)) >> (8 * (g & 1));
+    const uint32_t vx = *reinterpret_cast<const uint32_t*>(meta + 16 + (key & 12)) >> (8 * (g & 1));
+    const float ks[2] = {__uint_as_float(max((kx << 23) & 0x7f800000u, 0x00400000u)), __uint_as_float(max((kx << 7) & 0x7f800000u, 0x00400000u))};
+    const float vf[2] = {__uint_as_float(max((vx << 23) & 0x7f800000u, 0x00400000u)), __uint_as_float(max((vx << 7) & 0x7f800000u, 0x00400000u))};
+    const bool rare = __any_sync(0xffffffffu, j0 + 15 > least || max3f(ks[0], ks[1], fmaxf(vf[0], vf[1])) == INFINITY) || !ok;
+    const bool nan[2] = {fmaxf(ks[0], vf[0]) == INFINITY, fmaxf(ks[1], vf[1]) == INFINITY};
+    float p[RT][2][2], pv[RT][2][2];  // [key][row]
+    auto weigh = [&]() {  // returns whether a weight passes 2^8
+      float top = 0.f;
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float x = __fmaf_rn(s[rt][0][2 * r + e] + s[rt][1][2 * r + e], rs[rt][e] * ks[r], -m[rt][e]);
+            p[rt][r][e] = ex2_approx(x);
+            pv[rt][r][e] = p[rt][r][e] * (vf[r] * rho[rt][e]);
+          }
+      if (rare) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
           for (int r = 0; r < 2; ++r)
-            if (!ok || j0 + key + 2 * r > lim[rt][e]) x[rt][r][e] = -INFINITY;
-    }
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
+            for (int e = 0; e < 2; ++e)
+              if (!ok || j0 + key + 2 * r > lim[rt][e]) p[rt][r][e] = pv[rt][r][e] = 0.f;
+              else if (nan[r]) p[rt][r][e] = pv[rt][r][e] = __uint_as_float(0x7fc00000u);
+      }
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
+      for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          // a masked key's exponent may be any byte, NaN's too
-          y[rt][r][e] = x[rt][r][e] == -INFINITY ? -INFINITY : x[rt][r][e] + nv[r];
-          over |= x[rt][r][e] > m[rt][e] + 8.f || y[rt][r][e] > mv[rt][e] + 8.f;
-        }
-    if (__any_sync(0xffffffffu, over)) {  // raise the references to the maxima
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) top = max3f(top, p[rt][r][e], pv[rt][r][e]);
+      return top > 256.f;
+    };
+    if (__any_sync(0xffffffffu, weigh())) {  // raise the references to the maxima
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         float al[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float mx = fmaxf(x[rt][0][e], x[rt][1][e]), my = fmaxf(y[rt][0][e], y[rt][1][e]);
+          float mx = PAGED_NONE, my = PAGED_NONE;
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+            if (!rare || (ok && !nan[r] && j0 + key + 2 * r <= lim[rt][e])) {
+              const float x = (s[rt][0][2 * r + e] + s[rt][1][2 * r + e]) * (rs[rt][e] * ks[r]);
+              mx = fmaxf(mx, x);
+              my = fmaxf(my, x + __log2f(vf[r]));
+            }
 #pragma unroll
           for (int k = 4; k < 32; k <<= 1) {
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
@@ -388,8 +401,9 @@ __global__ void __launch_bounds__(128, PagedCfg<D, RT>::CTAS) paged_kernel(const
           }
           mx = fmaxf(mx, m[rt][e]);
           my = fmaxf(my, mv[rt][e]);
-          l[rt][e] *= ex2_approx(m[rt][e] - finite_or_zero(mx));
-          al[e] = ex2_approx(mv[rt][e] - finite_or_zero(my));
+          l[rt][e] *= ex2_approx(m[rt][e] - mx);
+          al[e] = ex2_approx(mv[rt][e] - my);
+          rho[rt][e] = ex2_approx(mx - my);
           m[rt][e] = mx;
           mv[rt][e] = my;
         }
@@ -398,17 +412,16 @@ __global__ void __launch_bounds__(128, PagedCfg<D, RT>::CTAS) paged_kernel(const
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[rt][j][e] *= al[e & 1];
       }
+      weigh();
     }
     uint32_t pb[RT][2];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      const float u[2] = {finite_or_zero(m[rt][0]), finite_or_zero(m[rt][1])};
-      const float uv[2] = {finite_or_zero(mv[rt][0]), finite_or_zero(mv[rt][1])};
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        l[rt][0] += ex2_approx(x[rt][r][0] - u[0]);
-        l[rt][1] += ex2_approx(x[rt][r][1] - u[1]);
-        pb[rt][r] = movmatrix(pack_f16(ex2_approx(y[rt][r][0] - uv[0]), ex2_approx(y[rt][r][1] - uv[1])));
+        l[rt][0] += p[rt][r][0];
+        l[rt][1] += p[rt][r][1];
+        pb[rt][r] = movmatrix(pack_f16(pv[rt][r][0], pv[rt][r][1]));
       }
     }
     // ---- o^T += V^T P^T
@@ -450,10 +463,10 @@ __global__ void __launch_bounds__(128, PagedCfg<D, RT>::CTAS) paged_kernel(const
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int r = rt * 8 + 2 * t + e;
-      float top = -INFINITY;
+      float top = PAGED_NONE;
 #pragma unroll
       for (int w = 0; w < C::WARPS; ++w) top = fmaxf(top, sm[w][1][r]);
-      const float f = ex2_approx(mv[rt][e] - finite_or_zero(top));
+      const float f = ex2_approx(mv[rt][e] - top);
       // a NaN weight stays NaN; a warp without visible keys adds zeros
 #pragma unroll
       for (int j = 0; j < D / 16; ++j) {
@@ -470,12 +483,12 @@ __global__ void __launch_bounds__(128, PagedCfg<D, RT>::CTAS) paged_kernel(const
   if (row < ROWS) {
     int b, mr;
     row_of(row, b, mr);
-    float top = -INFINITY, topv = -INFINITY, sum = 0.f;
+    float top = PAGED_NONE, topv = PAGED_NONE, sum = 0.f;
 #pragma unroll
     for (int w = 0; w < C::WARPS; ++w) top = fmaxf(top, sm[w][0][row]), topv = fmaxf(topv, sm[w][1][row]);
 #pragma unroll
-    for (int w = 0; w < C::WARPS; ++w) sum += sm[w][2][row] * ex2_approx(sm[w][0][row] - finite_or_zero(top));
-    const float fac = sum == 0.f ? 0.f : ex2_approx(finite_or_zero(topv) - finite_or_zero(top)) / sum;
+    for (int w = 0; w < C::WARPS; ++w) sum += sm[w][2][row] * ex2_approx(sm[w][0][row] - top);
+    const float fac = sum == 0.f ? 0.f : ex2_approx(topv - top) / sum;
     const float lse = sum == 0.f ? -INFINITY : top + log2f(sum);
     const long long at = (PRE ? a.splits + split : split) * rows + ((long long)b * a.H + h) * a.M + mr;
 #pragma unroll
