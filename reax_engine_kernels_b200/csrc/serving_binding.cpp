@@ -38,6 +38,11 @@ void last_dense(const char* name, const Tensor& t) {
   if (t.dim() > 0 && t.size(-1) > 1 && t.stride(-1) != 1)
     refuse(std::string(name) + ": the last dimension must be contiguous (stride " + std::to_string(t.stride(-1)) + ")");
 }
+// an output that a view repeats would be written by several CTAs at once
+void not_expanded(const char* name, const Tensor& t) {
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1 && t.stride(i) == 0) refuse(std::string(name) + ": an output's elements must not overlap");
+}
 void dense(const char* name, const Tensor& t) {
   if (!t.is_contiguous()) refuse(std::string(name) + " must be contiguous");
 }
@@ -57,7 +62,7 @@ struct Cache {
   const Tensor &k, &ke, &v, &ve;
 };
 
-int64_t check_cache(const Cache& c, int64_t H, int64_t D, at::Device dev) {
+int64_t check_cache(const Cache& c, int64_t H, int64_t D, at::Device dev, bool written = false) {
   want("cache.k", c.k, at::kFloat8_e4m3fn, {-1, H, -1, D}, dev);
   want("cache.v", c.v, at::kFloat8_e4m3fn, c.k.sizes(), dev);
   want("cache.ke", c.ke, at::kByte, c.k.sizes().slice(0, 3), dev);
@@ -68,10 +73,11 @@ int64_t check_cache(const Cache& c, int64_t H, int64_t D, at::Device dev) {
   if (page <= 0 || page % 16) refuse("the page size must be a multiple of 16, got " + std::to_string(page));
   if (c.k.stride(3) != 1 || c.k.stride(2) != D || c.ke.stride(2) != 1)
     refuse("the rows of a page and head must be contiguous");
+  if (written) not_expanded("cache", c.k), not_expanded("cache", c.ke);
   return page;
 }
 
-int64_t check_kv(const Tensor& k, const Tensor& v, const Cache& c, const Tensor& slots) {
+int64_t check_kv(const Tensor& k, const Tensor& v, const Cache& c, const Tensor& slots, bool written = false) {
   if (k.dim() != 3) refuse("k must be [T, H, D], got " + shape_of(k.sizes()));
   const int64_t T = k.size(0), H = k.size(1), D = k.size(2);
   const at::Device dev = k.device();
@@ -82,14 +88,14 @@ int64_t check_kv(const Tensor& k, const Tensor& v, const Cache& c, const Tensor&
   last_dense("k", k);
   last_dense("v", v);
   dense("slots", slots);
-  const int64_t page = check_cache(c, H, D, dev);
+  const int64_t page = check_cache(c, H, D, dev, written);
   on_cuda(k);
   return page;
 }
 
 int kv_write(const Tensor& k, const Tensor& v, const Tensor& ck, const Tensor& ke, const Tensor& cv, const Tensor& ve,
              const Tensor& slots) {
-  const int64_t page = check_kv(k, v, {ck, ke, cv, ve}, slots);
+  const int64_t page = check_kv(k, v, {ck, ke, cv, ve}, slots, /*written=*/true);
   const c10::cuda::CUDAGuard guard(k.device());
   return reax_kv_write(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), ck.data_ptr(), ke.data_ptr(),
                        cv.data_ptr(), ve.data_ptr(), ck.stride(0), ck.stride(1), ke.stride(0), ke.stride(1),
@@ -106,6 +112,8 @@ std::tuple<int, Tensor, Tensor> kv_read(const Tensor& ck, const Tensor& ke, cons
   };
   Tensor k = make(k_out), v = make(v_out);
   if (k.dim() == 3 && k.size(0) != slots.size(0)) refuse("k has another number of rows than slots");
+  not_expanded("k", k);
+  not_expanded("v", v);
   const int64_t page = check_kv(k, v, {ck, ke, cv, ve}, slots);
   const c10::cuda::CUDAGuard guard(k.device());
   const int rc = reax_kv_read(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), ck.data_ptr(),
@@ -141,6 +149,7 @@ std::tuple<int, Tensor> fmha_paged(const Tensor& q, const Tensor& ck, const Tens
   if (out_) {
     want("out", *out_, at::kBFloat16, {B, H, M, D}, dev);
     last_dense("out", *out_);
+    not_expanded("out", *out_);
   }
   last_dense("q", q);
   last_dense("table", table);

@@ -110,6 +110,17 @@ def test_delta_refusals(kw, words):
         delta(**kw)
 
 
+def test_expanded_outputs_are_refused():
+    k, v, s = kv()
+    with pytest.raises(ValueError, match="overlap"):
+        rk.kv_read(cache(), s, k[:1].expand(4, 2, 128), v)
+    one = cache(pages=1)
+    with pytest.raises(ValueError, match="overlap"):
+        rk.kv_write(k, v, rk.KvCache(*(t.view(torch.uint8).expand(3, *t.shape[1:]).view(t.dtype) for t in one)), s)
+    with pytest.raises(ValueError, match="overlap"):
+        paged(out=torch.zeros(1, 2, 4, 128, dtype=BF).expand(2, 2, 4, 128))
+
+
 def test_c_entry_refusals_launch_nothing():
     """Bad sizes, alignment and pointers come back as codes; sizes of zero as success.  No device is touched for the refused ones."""
     lib = abi.load("libreax_decode")
