@@ -555,7 +555,9 @@ __device__ __forceinline__ void tmem_ld_16x256b_x2(uint32_t taddr, uint32_t (&r)
       : "memory");
 }
 // Programmatic dependent launch: the next kernel's CTAs may start once every CTA of this one has come here (or left), and
-// wait for all of this one's results at their pdl_wait.
+// wait for all of this one's results at their pdl_wait.  A kernel that is launched so behind whatever the stream holds waits before its
+// first access; one that runs beside the kernel before it (whose CTAs have all waited by then) waits at its end instead, so
+// that what follows finds the results of both.
 __device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

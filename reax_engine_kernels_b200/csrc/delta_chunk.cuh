@@ -307,6 +307,7 @@ __device__ __forceinline__ int dc_sequence(const DeltaArgs& a) {
 __global__ void __launch_bounds__(DC_THREADS, 2) delta_chunk_kernel(DeltaArgs a) {
   extern __shared__ __align__(128) uint8_t dc_raw[];
   DcSmem& s = *reinterpret_cast<DcSmem*>(dc_raw);
+  pdl_wait();
   pdl_launch();  // the step kernel's sequences are others
   const int n = dc_sequence(a), hv = blockIdx.y, lane = threadIdx.x & 31, warp = warp_id();
   const int gq = lane >> 2, t4 = lane & 3, row0 = blockIdx.x * 64;
@@ -527,10 +528,8 @@ inline int delta_go(const reax::DeltaArgs& a, cudaStream_t st) {
   const dim3 grid(2, a.HV, a.N);
   // Each kernel takes the sequences of its lengths, which are on the device.  T = N is taken for a decode batch and T <= DS_MOST
   // leaves no long sequence: the step kernel alone then takes every length.
-  if (a.T == a.N || a.T <= reax::DS_MOST) {
-    reax::delta_step_kernel<<<grid, reax::DS_THREADS, 0, st>>>(a, 0x7fffffffffffffffLL);
-    return (int)cudaGetLastError();
-  }
+  if (a.T == a.N || a.T <= reax::DS_MOST)
+    return launch_dependent(reax::delta_step_kernel, grid, reax::DS_THREADS, 0, true, st, 1, a, 0x7fffffffffffffffLL, true);
   static SmemAttr attr;
   if (ensure_smem(attr, reax::delta_chunk_kernel, (int)sizeof(reax::DcSmem), true) != cudaSuccess) return -4;
   // setmaxnreg's shares (four warps of 168 registers a thread, four of 88) come out of the registers of the launch: with fewer
@@ -542,9 +541,8 @@ inline int delta_go(const reax::DeltaArgs& a, cudaStream_t st) {
     regs = at.numRegs;
   }
   if (regs < 128) return -4;
-  reax::delta_chunk_kernel<<<grid, reax::DC_THREADS, sizeof(reax::DcSmem), st>>>(a);
-  if (cudaError_t e = cudaGetLastError()) return (int)e;
-  return launch_dependent(reax::delta_step_kernel, grid, reax::DS_THREADS, 0, true, st, 1, a, reax::DS_MOST);
+  if (int rc = launch_dependent(reax::delta_chunk_kernel, grid, reax::DC_THREADS, (int)sizeof(reax::DcSmem), true, st, 1, a)) return rc;
+  return launch_dependent(reax::delta_step_kernel, grid, reax::DS_THREADS, 0, true, st, 1, a, reax::DS_MOST, false);
 }
 
 }  // namespace reax_host

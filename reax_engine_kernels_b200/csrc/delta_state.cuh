@@ -63,7 +63,8 @@ __device__ __forceinline__ int delta_slot(const DeltaArgs& a, int n) {
 }
 
 // grid (2, HV, N): 64 rows of one (sequence, value head) per CTA; sequences of more than `most` tokens are the chunk kernel's
-__global__ void __launch_bounds__(DS_THREADS) delta_step_kernel(DeltaArgs a, long long most) {
+__global__ void __launch_bounds__(DS_THREADS) delta_step_kernel(DeltaArgs a, long long most, bool first) {
+  if (first) pdl_wait();
   const int n = blockIdx.z, hv = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int sub = lane & 15, half = lane >> 4, own = sub >> 1;
   const int row0 = blockIdx.x * 64 + warp * 16 + half * 8;

@@ -77,6 +77,7 @@ __global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(KvArgs a) {
   const uint16_t* src = (is_v ? a.v : a.k) + h * (is_v ? a.vH : a.sH) + sub * 16;
   const long long sT = is_v ? a.vT : a.sT;
   const long long t0 = (long long)blockIdx.x * (RPB * R) + row;
+  pdl_wait();
   uint4 x[R][2];
   long long at[R];
 #pragma unroll
@@ -137,6 +138,7 @@ __global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(KvArgs a) {
   uint16_t* dst = (is_v ? a.vo : a.ko) + h * (is_v ? a.vH : a.sH) + sub * 16;
   const long long sT = is_v ? a.vT : a.sT;
   const long long t0 = (long long)blockIdx.x * (RPB * R) + row;
+  pdl_wait();
   long long at[R];
   uint4 x[R];
   uint32_t ex[R];
@@ -202,14 +204,9 @@ inline int kv_go(const reax::KvArgs& a, int H, cudaStream_t st) {
   const long long wide = (long long)((a.T + RPB * R - 1) / (RPB * R)) * H * 2;
   const int r = wide >= 2LL * device_sms(dev) ? R : 1;
   const dim3 grid((a.T + RPB * r - 1) / (RPB * r), H, 2);
-  if (WRITE) {
-    if (r == 1) reax::kv_write_kernel<D, 1><<<grid, reax::KV_THREADS, 0, st>>>(a);
-    else reax::kv_write_kernel<D, R><<<grid, reax::KV_THREADS, 0, st>>>(a);
-  } else {
-    if (r == 1) reax::kv_read_kernel<D, 1><<<grid, reax::KV_THREADS, 0, st>>>(a);
-    else reax::kv_read_kernel<D, R><<<grid, reax::KV_THREADS, 0, st>>>(a);
-  }
-  return (int)cudaGetLastError();
+  void (*kernel)(reax::KvArgs) = WRITE ? (r == 1 ? reax::kv_write_kernel<D, 1> : reax::kv_write_kernel<D, R>)
+                                       : (r == 1 ? reax::kv_read_kernel<D, 1> : reax::kv_read_kernel<D, R>);
+  return launch_dependent(kernel, grid, reax::KV_THREADS, 0, true, st, 1, a);
 }
 
 }  // namespace reax_host

@@ -182,6 +182,8 @@ __global__ void __launch_bounds__(128, PagedCfg<D, RT>::CTAS) paged_kernel(const
   __shared__ float srow[ROWS];
   __shared__ float sm[C::WARPS][3][ROWS];
   __shared__ float slse[ROWS];
+  if (PRE || a.psplits == 0) pdl_wait();  // beside a prefix kernel, that one has waited
+  if (PRE) pdl_launch();
   const int nsplit = PRE ? a.psplits : a.splits;
   const int h = blockIdx.y, split = blockIdx.x % nsplit, r0 = blockIdx.x / nsplit * ROWS;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -440,7 +442,7 @@ __global__ void __launch_bounds__(128, PagedCfg<D, RT>::CTAS) paged_kernel(const
     __syncwarp();  // the stage may be filled again
   }
   cp_async_wait<0>();
-  pdl_launch();
+  if (!PRE) pdl_launch();
 
   // ---- merge the four warps
 #pragma unroll

@@ -68,7 +68,7 @@ inline int paged_launch(const reax::PagedArgs& a, cudaStream_t st) {
   const long long x = PRE ? (long long)ceil_div((long long)a.B * a.M, C::ROWS) * a.psplits : (long long)ceil_div(a.M, C::ROWS) * a.splits;
   if (x > 0x7fffffffLL) return -1;
   const dim3 grid((unsigned)x, a.H, PRE ? 1 : a.B);
-  return launch_dependent(reax::paged_kernel<D, RT, PRE>, grid, 128, C::SMEM, !PRE && a.psplits, st, !PRE && a.cluster ? a.splits : 1, a);
+  return launch_dependent(reax::paged_kernel<D, RT, PRE>, grid, 128, C::SMEM, true, st, !PRE && a.cluster ? a.splits : 1, a);
 }
 
 template <int D>
@@ -78,8 +78,7 @@ inline int prefix_launch(const reax::PagedArgs& a, cudaStream_t st) {
   if (ensure_smem(attr, reax::prefix_kernel<D>, C::SMEM, true) != cudaSuccess) return -4;
   const long long x = (long long)ceil_div((long long)a.B * a.M, reax::PF_ROWS) * a.psplits;
   if (x > 0x7fffffffLL) return -1;
-  reax::prefix_kernel<D><<<dim3((unsigned)x, a.H), reax::PF_THREADS, C::SMEM, st>>>(a);
-  return (int)cudaGetLastError();
+  return launch_dependent(reax::prefix_kernel<D>, dim3((unsigned)x, a.H), reax::PF_THREADS, C::SMEM, true, st, 1, a);
 }
 
 // Up to 8 rows per (sequence, head), what a decode step has, go in one group of 8; more in CTAs of 16 rows.

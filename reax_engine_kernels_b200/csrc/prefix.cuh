@@ -66,6 +66,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
   __shared__ int abort_flag;
   __shared__ int skn[4], svn[4];          // a tile's largest nk and nv
   __shared__ uint32_t seven[4], sodd[4];  // its even and odd keys that exist
+  pdl_wait();
   pdl_launch();  // the own keys' kernel needs nothing from here
   const uint32_t base = (smem_u32(pf_raw) + 1023u) & ~1023u;
   const uint32_t sk = base, sv = sk + 2 * C::KV_BYTES, sraw = sv + 2 * C::KV_BYTES, sexp = sraw + C::NR * C::RAW;
