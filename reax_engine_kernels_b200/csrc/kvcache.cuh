@@ -217,7 +217,8 @@ inline int kv_go(const reax::KvArgs& a, int H, cudaStream_t st) {
                              long long esH, const long long* slots, int T, int H, int D, int page, long long pages,      \
                              void* stream) {                                                                            \
     reax::KvArgs a{(const uint16_t*)k, (const uint16_t*)v, nullptr, nullptr, ksT, ksH, vsT, vsH, (uint8_t*)kc,             \
-                   (uint8_t*)ke, (uint8_t*)vc, (uint8_t*)ve, csP, csH, esP, esH, slots, pages * page, T, page, reax_host::page_shift(page)};            \
+                   (uint8_t*)ke, (uint8_t*)vc, (uint8_t*)ve, csP, csH, esP, esH, slots, pages * page, T, page,                    \
+                   reax_host::page_shift(page)};                                                                          \
     if (int rc = reax_host::kv_check(a, k, v, H, D, pages)) return rc;                                                    \
     return D == 128 ? reax_host::kv_go<true, 128>(a, H, (cudaStream_t)stream)                                             \
                     : reax_host::kv_go<true, 256>(a, H, (cudaStream_t)stream);                                            \
@@ -227,7 +228,8 @@ inline int kv_go(const reax::KvArgs& a, int H, cudaStream_t st) {
                             long long esH, const long long* slots, int T, int H, int D, int page, long long pages,       \
                             void* stream) {                                                                             \
     reax::KvArgs a{nullptr, nullptr, (uint16_t*)k, (uint16_t*)v, ksT, ksH, vsT, vsH, (uint8_t*)kc, (uint8_t*)ke,           \
-                   (uint8_t*)vc, (uint8_t*)ve, csP, csH, esP, esH, slots, pages * page, T, page, reax_host::page_shift(page)};                          \
+                   (uint8_t*)vc, (uint8_t*)ve, csP, csH, esP, esH, slots, pages * page, T, page,                                  \
+                   reax_host::page_shift(page)};                                                                          \
     if (int rc = reax_host::kv_check(a, k, v, H, D, pages)) return rc;                                                    \
     return D == 128 ? reax_host::kv_go<false, 128>(a, H, (cudaStream_t)stream)                                            \
                     : reax_host::kv_go<false, 256>(a, H, (cudaStream_t)stream);                                           \

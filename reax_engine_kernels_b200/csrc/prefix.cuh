@@ -10,17 +10,21 @@
 //   13      bulk copies of the cache's bytes, 16 rows (always in one page) at a time, up to two (four) tiles ahead.  (Loads into
 //           registers by the dequantising warps took longer to issue than the conversion: 159 us for the shared document.)
 //   12      one thread issues S_j = Q K_j^T (M = 128, N = 64, K = D), then O += P_{j-1} V_{j-1} (N = D, K = 64).
-// K and V have two buffers each, S two, freed by tcgen05.commit.  The products of a tile take about 1100 cycles of the tensor pipe at
-// D = 256, the conversions about 400 of the ALU's, the exponents 512 of the MUFU's; what they share is the shared-memory
-// port, where the f16 rows are written and read once (1024 cycles) and the cache's bytes pass.  So q and P are operands out of
-// tensor memory (q out of shared memory would be another 512 cycles a tile).
+// K and V have two buffers each, S two, freed by tcgen05.commit.
+//
+// At D = 256 a tile takes 2430 cycles: S is a chain of 16 dependent products (1400 cycles, 32 of arithmetic each), PV four (730), the
+// conversion 1700 on eight warps, the softmax 1660 on four, all side by side.  What they share is the shared-memory port, where
+// the f16 rows are written and read once (1024 cycles) and the cache's bytes pass; so q and P are operands out of tensor
+// memory.  64 questions on a shared document of 32768 tokens: 136 us.  Measured slower: tiles of 128 keys, whose f16 rows leave
+// room for one buffer each (186 us); S as two chains side by side, which leaves q no room in tensor memory (157 us).
 //
 // The rows' powers of two go into the f16 values, relative to the tile's largest (nk, nv): e4m3 has 4 bits, f16 11, and a row stays
-// exact down to 2^-12 of the tile's largest row, and right to 2^-12 of its own largest value down to 2^-20.  What is
+// exact down to 2^-15 of the tile's largest row, and right to 2^-13 of its own largest value down to 2^-20.  What is
 // left is one factor per tile, so a score costs one multiply-add and one exponent: P = 2^(x - m + nv - ref + 7), ref the
 // running maximum of the tiles' nv, m a lazy maximum that no x passes by more than 8 (P < 2^15).  The 7 keeps f16's
-// full precision down to 2^-21.  (Raising m costs a pass over O in tensor memory: with 2 in place of the 8 most tiles did.)  (Both powers of two applied to the scores, as paged_kernel does it, made the softmax the
-// bound: 254 us for 64 questions on a shared document of 32768 tokens.)  O carries 2^-ref and 2^7 until the end.
+// full precision down to 2^-21.  (Raising m costs a pass over O in tensor memory: with 2 in place of the 8 most tiles did.
+// Both powers of two applied to the scores, with two exponents each, made the softmax the bound: 254 us.)  O carries 2^-ref
+// and 2^7 until the end.
 // A row whose K or V is NaN becomes a NaN key and a zero value, which reaches the queries that see it and no others.
 #pragma once
 #include "paged.cuh"

@@ -24,10 +24,12 @@ std::string shape_of(at::IntArrayRef s) {
 
 // `t` has that dtype, device and shape (a size of -1: any)
 void want(const char* name, const Tensor& t, at::ScalarType dtype, at::IntArrayRef shape, at::Device device) {
-  if (t.scalar_type() != dtype)
-    refuse(std::string(name) + " must be torch." + (dtype == at::kBFloat16 ? "bfloat16" : dtype == at::kFloat ? "float32" : dtype == at::kInt ? "int32"
-           : dtype == at::kLong ? "int64" : dtype == at::kByte ? "uint8" : dtype == at::kBool ? "bool" : "float8_e4m3fn") +
-           ", got " + std::string(at::toString(t.scalar_type())));
+  if (t.scalar_type() != dtype) {
+    const char* wanted = dtype == at::kBFloat16 ? "bfloat16" : dtype == at::kFloat ? "float32" : dtype == at::kInt ? "int32"
+                         : dtype == at::kLong   ? "int64"    : dtype == at::kByte ? "uint8"   : dtype == at::kBool ? "bool"
+                                                                                                                   : "float8_e4m3fn";
+    refuse(std::string(name) + " must be torch." + wanted + ", got " + std::string(at::toString(t.scalar_type())));
+  }
   if (t.device() != device) refuse(std::string(name) + " is on " + t.device().str() + ", the operands on " + device.str());
   bool same = t.dim() == (int64_t)shape.size();
   for (size_t i = 0; same && i < shape.size(); ++i) same = shape[i] < 0 || shape[i] == t.size(i);
