@@ -11,8 +11,8 @@
 //
 // HBM-bound: 2 D bytes read and D + 1 written per row (write), the reverse (read).  A thread owns 16 values (two 16-byte
 // loads, one 16-byte store), D / 16 lanes share a row; a CTA handles consecutive tokens of one head, so that its stores
-// fall in whole pages, and a thread has up to R = 2 rows in flight (four: fewer CTAs fit, 73 us for the write below).  32768
-// tokens x 8 heads of 256: written in 63 us, read back in 67, 6.2 and 6.0 TB/s.
+// fall in whole pages.  One row a thread; two in a large write (four: fewer CTAs fit, 73 us for the write below).  32768
+// tokens x 8 heads of 256: written in 61 us, read back in 66, 6.4 and 6.0 TB/s.
 #pragma once
 #include "common.cuh"
 
@@ -87,8 +87,8 @@ __global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(KvArgs a) {
     x[i][0] = x[i][1] = make_uint4(0, 0, 0, 0);
     if (t < a.T) {
       const uint4* p = reinterpret_cast<const uint4*>(src + t * sT);
-      x[i][0] = __ldg(p);
-      x[i][1] = __ldg(p + 1);
+      x[i][0] = *p;
+      x[i][1] = p[1];
       at[i] = kv_slot(a, (int)t);
     }
   }
@@ -130,50 +130,35 @@ __device__ __forceinline__ uint32_t dequant2(uint32_t two, float scale) {
   return pack_bf16(lo * scale, hi * scale);
 }
 
-template <int D, int R>
+// grid (token tiles, H, 2: k / v)
+template <int D>
 __global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(KvArgs a) {
   constexpr int LPR = D / 16, RPB = KV_THREADS / LPR;
-  const int sub = threadIdx.x % LPR, row = threadIdx.x / LPR, h = blockIdx.y;
+  const int sub = threadIdx.x % LPR, h = blockIdx.y;
   const bool is_v = blockIdx.z;
-  uint16_t* dst = (is_v ? a.vo : a.ko) + h * (is_v ? a.vH : a.sH) + sub * 16;
-  const long long sT = is_v ? a.vT : a.sT;
-  const long long t0 = (long long)blockIdx.x * (RPB * R) + row;
+  const long long t = (long long)blockIdx.x * RPB + threadIdx.x / LPR;
   pdl_wait();
-  long long at[R];
-  uint4 x[R];
-  uint32_t ex[R];
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const long long t = t0 + i * RPB;
-    at[i] = t < a.T ? kv_slot(a, (int)t) : -1;
+  if (t >= a.T) return;
+  const long long at = kv_slot(a, (int)t);
+  uint4 x = make_uint4(0, 0, 0, 0);
+  uint32_t ex = 0;
+  if (at >= 0) {
+    int off;
+    const long long pg = kv_page(a, at, off);
+    x = __ldcs(reinterpret_cast<const uint4*>((is_v ? a.vc : a.kc) + pg * a.cP + h * a.cH + (long long)off * D + sub * 16));
+    ex = ((is_v ? a.ve : a.ke) + pg * a.eP + h * a.eH)[off];
   }
+  const float s = pow2_byte(ex);
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  uint32_t y[8];
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    x[i] = make_uint4(0, 0, 0, 0);
-    ex[i] = 0;
-    if (at[i] >= 0) {
-      int off;
-      const long long pg = kv_page(a, at[i], off);
-      x[i] = __ldcs(reinterpret_cast<const uint4*>((is_v ? a.vc : a.kc) + pg * a.cP + h * a.cH + (long long)off * D + sub * 16));
-      ex[i] = ((is_v ? a.ve : a.ke) + pg * a.eP + h * a.eH)[off];
-    }
+  for (int j = 0; j < 4; ++j) {
+    y[2 * j] = dequant2(w[j] & 0xffffu, s);
+    y[2 * j + 1] = dequant2(w[j] >> 16, s);
   }
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const long long t = t0 + i * RPB;
-    if (t >= a.T) continue;
-    const float s = pow2_byte(ex[i]);
-    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-    uint32_t y[8];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      y[2 * j] = dequant2(w[j] & 0xffffu, s);
-      y[2 * j + 1] = dequant2(w[j] >> 16, s);
-    }
-    uint4* p = reinterpret_cast<uint4*>(dst + t * sT);
-    __stcs(p, make_uint4(y[0], y[1], y[2], y[3]));
-    __stcs(p + 1, make_uint4(y[4], y[5], y[6], y[7]));
-  }
+  uint4* p = reinterpret_cast<uint4*>((is_v ? a.vo : a.ko) + t * (is_v ? a.vT : a.sT) + h * (is_v ? a.vH : a.sH) + sub * 16);
+  __stcs(p, make_uint4(y[0], y[1], y[2], y[3]));
+  __stcs(p + 1, make_uint4(y[4], y[5], y[6], y[7]));
 }
 
 }  // namespace reax
@@ -197,15 +182,14 @@ inline int kv_check(const reax::KvArgs& a, const void* x, const void* y, int H, 
 template <bool WRITE, int D>
 inline int kv_go(const reax::KvArgs& a, int H, cudaStream_t st) {
   if (a.T == 0) return 0;
-  constexpr int RPB = reax::KV_THREADS / (D / 16), R = 2;
+  constexpr int RPB = reax::KV_THREADS / (D / 16);
   int dev = 0;
   cudaGetDevice(&dev);
-  // two rows a thread once that still gives every SM two CTAs; below it, one row a thread for the shorter chain
-  const long long wide = (long long)((a.T + RPB * R - 1) / (RPB * R)) * H * 2;
-  const int r = wide >= 2LL * device_sms(dev) ? R : 1;
+  // The write takes two rows a thread from ten waves of CTAs on (16 fit an SM), where HBM is the bound: 32768 tokens x 8 heads of 256
+  // in 61.4 us, 64.5 with one; 8192 x 8 heads of 128, which the L2 takes in, in 9.9 with one, 10.5 with two.
+  const int r = WRITE && (long long)((a.T + RPB - 1) / RPB) * H * 2 > 160LL * device_sms(dev) ? 2 : 1;
   const dim3 grid((a.T + RPB * r - 1) / (RPB * r), H, 2);
-  void (*kernel)(reax::KvArgs) = WRITE ? (r == 1 ? reax::kv_write_kernel<D, 1> : reax::kv_write_kernel<D, R>)
-                                       : (r == 1 ? reax::kv_read_kernel<D, 1> : reax::kv_read_kernel<D, R>);
+  void (*kernel)(reax::KvArgs) = !WRITE ? reax::kv_read_kernel<D> : r == 1 ? reax::kv_write_kernel<D, 1> : reax::kv_write_kernel<D, 2>;
   return launch_dependent(kernel, grid, reax::KV_THREADS, 0, true, st, 1, a);
 }
 

@@ -133,6 +133,24 @@ def test_cache_written_and_read(T, H, D, page, fused):
         assert torch.equal(torch.nan_to_num(got, nan=7.0), torch.nan_to_num(want, nan=7.0))
 
 
+def test_large_write_two_rows_a_thread():
+    """Past ten waves of CTAs a thread writes two rows: the same codes as in parts that do not reach it."""
+    T, H, D, page = 12501 * torch.cuda.get_device_properties(0).multi_processor_count // 148, 8, 256, 16
+    g = gen(77)
+    k, v = randn(g, T, H, D).to(BF), odd_rows(g, T, H, D)
+    slots = torch.randperm(-(-T // page) * page, generator=g, device=DEV)[:T].contiguous()
+    slots[T // 3] = -1
+    a, b = (rk.kv_cache(-(-T // page), H, page, D) for _ in range(2))
+    rk.kv_write(k, v, a, slots)
+    for i in range(0, T, 1000):
+        rk.kv_write(k[i:i + 1000], v[i:i + 1000], b, slots[i:i + 1000])
+    for x, y in zip(a, b):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+    wc, we = quantise_ref(v[-50:])
+    at = slots[-50:]
+    assert torch.equal(a.v.view(torch.uint8)[at // page, :, at % page].cpu(), wc) and torch.equal(a.ve[at // page, :, at % page].cpu(), we)
+
+
 def test_slots_past_the_end_are_skipped_and_reported():
     g = gen(5)
     k = randn(g, 4, 2, 128).to(BF)
@@ -402,6 +420,64 @@ def test_graph_replays_with_other_lengths_and_two_graphs_share_nothing():
         # without the prefix these positions reach past a history's pages, to entries of -5: reported, not seen
         assert_attention(outs[0], q, c, table, 0.1, qpos, 4, bad=(-5,))
     status()
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_inputs_made_on_another_stream(captured):
+    """The kernels start as dependents of what their stream holds before them: what another stream made, joined by an event, is
+    waited for all the same, and so is the consumer on a third stream for them."""
+    B, H, G, D, page, L = 3, 2, 4, 128, 16, 200
+    q0, c, table, qpos, prefix = setup(31, B, H, G, 1, D, page, [L] * B, 100)
+    g = gen(32)
+    k0, v0 = randn(g, B, H, D).to(BF), randn(g, B, H, D).to(BF)
+    slots = table.long()[torch.arange(B, device=DEV), (L - 1) // page] * page + (L - 1) % page
+    d = delta_inputs(33, [1, 40, 16], 2, 4, 3)
+    st0 = d["state"].clone()
+    q, k, v, dk = (torch.zeros_like(x) for x in (q0, k0, v0, d["k"]))
+    big = torch.randn(4096, 4096, device=DEV)
+    out = {}
+
+    def run():
+        main, s1, s2 = torch.cuda.current_stream(), torch.cuda.Stream(), torch.cuda.Stream()
+        s1.wait_stream(main)
+        with torch.cuda.stream(s1):  # a producer that takes a while
+            x = big
+            for _ in range(6):
+                x = x @ big * 1e-2
+            for dst, src in ((q, q0), (k, k0), (v, v0), (dk, d["k"])):
+                dst.copy_(src)
+            d["state"].copy_(st0)
+        scratch = big[0] * 2  # a kernel of this stream's own just before the join
+        main.wait_stream(s1)
+        rk.kv_write(k, v, c, slots)
+        o = rk.fmha_paged(q, c, table, D ** -0.5, qpos=qpos, G=G, prefix=prefix, prefix_len=100)
+        r = rk.delta_state(d["q"], dk, d["v"], d["g"], d["beta"], d["cu"], 0.1, d["state"])
+        s2.wait_stream(main)
+        with torch.cuda.stream(s2):
+            out["o"], out["r"] = o.clone(), r.clone()
+        main.wait_stream(s2)
+        out["keep"] = (x, scratch, o, r)
+
+    if captured:
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            run()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run()
+    for _ in range(3):
+        for x in (q, k, v, dk):
+            x.zero_()
+        torch.cuda.synchronize()
+        graph.replay() if captured else run()
+        torch.cuda.synchronize()
+        state = d["state"].clone()
+        rk.kv_write(k0, v0, c, slots)
+        o = rk.fmha_paged(q0, c, table, D ** -0.5, qpos=qpos, G=G, prefix=prefix, prefix_len=100)
+        d["state"].copy_(st0)
+        r = rk.delta_state(d["q"], d["k"], d["v"], d["g"], d["beta"], d["cu"], 0.1, d["state"])
+        assert torch.equal(out["o"], o) and torch.equal(out["r"], r) and torch.equal(state, d["state"])
 
 
 def test_same_bits_every_time():
