@@ -527,7 +527,8 @@ inline int delta_go(const reax::DeltaArgs& a, cudaStream_t st) {
   if (a.N == 0 || a.T == 0) return 0;
   const dim3 grid(2, a.HV, a.N);
   // Each kernel takes the sequences of its lengths, which are on the device.  T = N is taken for a decode batch and T <= DS_MOST
-  // leaves no long sequence: the step kernel alone then takes every length.
+  // leaves no long sequence: the step kernel alone then takes every length.  (64 sequences of one token, 32 heads: 48 us; with the
+  // chunk kernel, which finds nothing to do, beside it 74.)
   if (a.T == a.N || a.T <= reax::DS_MOST)
     return launch_dependent(reax::delta_step_kernel, grid, reax::DS_THREADS, 0, true, st, 1, a, 0x7fffffffffffffffLL, true);
   static SmemAttr attr;
