@@ -96,7 +96,7 @@ def build_binding(force: bool = False) -> str:
     tmp = out + ".tmp"
     cmd = (["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"] + [f"-I{p}" for p in inc] + [src, "-o", tmp, f"-L{LIBDIR}",
-            "-l:libreax_decode.so", f"-L{torch_lib}", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"])
+            "-l:libreax_decode.so", f"-L{torch_lib}", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"])
     _run(cmd, "_serving")
     os.replace(tmp, out)
     return out

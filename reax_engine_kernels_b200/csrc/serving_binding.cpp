@@ -3,6 +3,7 @@
 // Python with a ctypes call cost more than that: a 64-token kv_write took 22.2 us a call, with this binding 4.1 us.
 //
 // Refused arguments raise ValueError before any device is touched; the functions return the C entry point's code.
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -58,6 +59,10 @@ int to_int(const char* name, int64_t n) {
   if (n < 0 || n > 0x7fffffff) refuse(std::string(name) + " = " + std::to_string(n) + " is out of range");
   return (int)n;
 }
+// straight from the caching allocator, without the dispatcher's share of a microsecond
+Tensor empty_on(at::IntArrayRef shape, at::ScalarType dtype, at::Device device) {
+  return Tensor(at::detail::empty_cuda(shape, dtype, device, std::nullopt));
+}
 void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
 struct Cache {
@@ -109,8 +114,9 @@ std::tuple<int, Tensor, Tensor> kv_read(const Tensor& ck, const Tensor& ke, cons
                                         const Tensor& slots, const OptTensor& k_out, const OptTensor& v_out) {
   if (ck.dim() != 4 || slots.dim() != 1)
     refuse("cache.k must be [pages, H, page, D] and slots [T], got " + shape_of(ck.sizes()) + ", " + shape_of(slots.sizes()));
+  if (!k_out || !v_out) on_cuda(slots);
   const auto make = [&](const OptTensor& t) {
-    return t ? *t : at::empty({slots.size(0), ck.size(1), ck.size(3)}, slots.options().dtype(at::kBFloat16));
+    return t ? *t : empty_on({slots.size(0), ck.size(1), ck.size(3)}, at::kBFloat16, slots.device());
   };
   Tensor k = make(k_out), v = make(v_out);
   if (k.dim() == 3 && k.size(0) != slots.size(0)) refuse("k has another number of rows than slots");
@@ -157,14 +163,14 @@ std::tuple<int, Tensor> fmha_paged(const Tensor& q, const Tensor& ck, const Tens
   last_dense("table", table);
   last_dense("qpos", qpos);
   on_cuda(q);
-  Tensor out = out_ ? *out_ : at::empty({B, H, M, D}, q.options());
+  Tensor out = out_ ? *out_ : empty_on({B, H, M, D}, at::kBFloat16, dev);
   const c10::cuda::CUDAGuard guard(dev);
   const int b = to_int("B", B), h = to_int("H", H), m = to_int("M", M), d = (int)D, P = to_int("P", table.size(1)),
             pg = to_int("page", page), Lp = to_int("prefix_len", prefix_len);
   const int splits = reax_fmha_paged_splits(b, h, m, d, P, pg, Lp);
   if (splits < 0) return {splits, out};
   Tensor ws;
-  if (splits > 1 && B && M) ws = at::empty({splits * B * H * M * (D + 1)}, q.options().dtype(at::kFloat));
+  if (splits > 1 && B && M) ws = empty_on({splits * B * H * M * (D + 1)}, at::kFloat, dev);
   const int rc = reax_fmha_paged(
       q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), ck.data_ptr(), ke.data_ptr(), cv.data_ptr(), ve.data_ptr(), ck.stride(0),
       ck.stride(1), ke.stride(0), ke.stride(1), (const int*)table.data_ptr(), table.stride(0),
@@ -215,7 +221,7 @@ std::tuple<int, Tensor> delta_state(const Tensor& q, const Tensor& k, const Tens
   dense("g", g);
   dense("cu", cu);
   on_cuda(q);
-  Tensor o = o_ ? *o_ : at::empty({T, HV, 128}, q.options());
+  Tensor o = o_ ? *o_ : empty_on({T, HV, 128}, at::kBFloat16, dev);
   const c10::cuda::CUDAGuard guard(dev);
   const int rc = reax_delta_state(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), (const long long*)cu.data_ptr(),
                                   state.data_ptr(), state.stride(0), slots ? (const int*)slots->data_ptr() : nullptr,
