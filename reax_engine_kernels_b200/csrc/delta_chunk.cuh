@@ -315,9 +315,9 @@ __global__ void __launch_bounds__(DC_THREADS, 2) delta_chunk_kernel(DeltaArgs a)
   delta_range(a, n, t0, e);
   if (e - t0 <= DS_MOST) return;
   const int slot = delta_slot(a, n);
-  if (slot == -1) return;
+  if (slot < 0) return;
   const long long oT = (long long)a.HV * 128;
-  if (slot < 0) {  // the rows of a sequence that cannot run are NaN
+  if (!delta_slot_ok(a, n, slot)) {  // the rows of a sequence that cannot run are NaN
     uint16_t* o = a.o + (long long)hv * 128 + row0;
     for (long long i = threadIdx.x; i < (e - t0) * 64; i += DC_THREADS) o[(t0 + (i >> 6)) * oT + (i & 63)] = 0x7fff;
     return;
@@ -527,8 +527,8 @@ inline int delta_go(const reax::DeltaArgs& a, cudaStream_t st) {
   if (a.N == 0 || a.T == 0) return 0;
   const dim3 grid(2, a.HV, a.N);
   // Each kernel takes the sequences of its lengths, which are on the device.  T = N is taken for a decode batch and T <= DS_MOST
-  // leaves no long sequence: the step kernel alone then takes every length.  (64 sequences of one token, 32 heads: 48 us; with the
-  // chunk kernel, which finds nothing to do, beside it 74.)
+  // leaves no long sequence: the step kernel alone then takes every length.  (64 sequences of one token, 32 heads: 45 us; with the
+  // chunk kernel, which finds nothing to do, beside it 73.)
   if (a.T == a.N || a.T <= reax::DS_MOST)
     return launch_dependent(reax::delta_step_kernel, grid, reax::DS_THREADS, 0, true, st, 1, a, 0x7fffffffffffffffLL, true);
   static SmemAttr attr;
