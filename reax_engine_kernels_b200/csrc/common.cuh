@@ -130,11 +130,20 @@ __device__ __forceinline__ void mbar_arrive_expect_tx(uint32_t bar, uint32_t byt
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// REAX_WAIT_POLL (a test build): every look at a barrier returns at once.  try_wait suspends for microseconds before it
+// reports that a phase is not there, so a limit shorter than that would never be seen to pass.
+#ifdef REAX_WAIT_POLL
+#define REAX_MBAR_LOOK "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+#define REAX_MBAR_LOOK_NS REAX_MBAR_LOOK
+#else
+#define REAX_MBAR_LOOK "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+#define REAX_MBAR_LOOK_NS "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+#endif
 __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      REAX_MBAR_LOOK
       "selp.u32 %0, 1, 0, p;\n\t}\n"
       : "=r"(ok)
       : "r"(bar), "r"(parity)
@@ -147,7 +156,7 @@ __device__ __forceinline__ bool mbar_try_wait_sleep(uint32_t bar, uint32_t parit
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      REAX_MBAR_LOOK_NS
       "selp.u32 %0, 1, 0, p;\n\t}\n"
       : "=r"(ok)
       : "r"(bar), "r"(parity), "r"(ns)

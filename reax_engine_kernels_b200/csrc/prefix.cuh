@@ -4,26 +4,30 @@
 // keys, and the prefix is read (and dequantised) once per 128 rows instead of once per sequence.  The result is a partial output
 // and the log2 of its sum for each row and chunk of the prefix, as paged_kernel leaves them; paged_join_kernel joins all.
 //
-// One CTA per SM takes 128 rows of one head and a chunk of the keys, 64 at a time.  14 warps:
+// One CTA per SM takes 128 rows of one head and a chunk of the keys, 64 at a time.  15 warps:
 //   0..3    softmax, a thread per row (TMEM lane): S out of TMEM, P (f16) back over it;
-//   4..11   dequantisation: 16 cache bytes -> 16 f16 in 128-byte-swizzled shared memory, each warp eight rows of K and of V per tile;
-//   13      bulk copies of the cache's bytes, 16 rows (always in one page) at a time, up to two (four) tiles ahead.  (Loads into
-//           registers by the dequantising warps took longer to issue than the conversion: 159 us for the shared document.)
-//   12      one thread issues S_j = Q K_j^T (M = 128, N = 64, K = D), then O += P_{j-1} V_{j-1} (N = D, K = 64).
+//   4..7    dequantisation of K: 16 cache bytes -> 16 f16 in 128-byte-swizzled shared memory, each warp sixteen rows of a tile;
+//   8..11   of V.  (All eight on K, then on V: each waits on both sides of either, and 126 us where these take 123.)
+//   13, 14  bulk copies of the bytes of K, of V, as many rows at a time as surely lie in one page (16 to 64), three tiles ahead (four
+//           at D = 128).  (Loads into registers by the dequantising warps took longer to issue than the conversion; one warp for both
+//           copies is late with pages of 16: 70 us for a call that takes 62, 32 questions on 32768 tokens in heads of 256.)
+//   12      issues S_j = Q K_j^T (M = 128, N = 64, K = D), then O += P_{j-1} V_{j-1} (N = D, K = 64).
 // K and V have two buffers each, S two, freed by tcgen05.commit.
 //
-// At D = 256 a tile takes 2430 cycles: S is a chain of 16 dependent products (1400 cycles, 32 of arithmetic each), PV four (730), the
-// conversion 1700 on eight warps, the softmax 1660 on four, all side by side.  What they share is the shared-memory port, where
-// the f16 rows are written and read once (1024 cycles) and the cache's bytes pass; so q and P are operands out of tensor
-// memory.  64 questions on a shared document of 32768 tokens: 136 us.  Measured slower: tiles of 128 keys, whose f16 rows leave
-// room for one buffer each (186 us); S as two chains side by side, which leaves q no room in tensor memory (157 us).
+// At D = 256 a tile takes 2150 cycles, what the softmax's four warps take from S to P (750 to read it and for the maximum, 1050 for 64
+// exponents a thread and P, the rest waits); the products 530 and 510 (the tensor core's rate), the conversions 1500 each, side by side.
+// What they share is the shared-memory port, where the f16 rows are written and read once (1024 cycles) and the cache's bytes pass; so q
+// and P are operands out of tensor memory.  64 questions on a shared document of 32768 tokens: 123 us, 78 of them here.  Measured
+// slower: a branch of one lane to issue the products (137 us), tiles of 128 keys, whose f16 rows leave room for one buffer each; S
+// as two chains side by side, which leaves q no room in tensor memory; a half to an eighth of the exponents as polynomials on the FMA
+// pipe (128 to 123.5).
 //
 // The rows' powers of two go into the f16 values, relative to the tile's largest (nk, nv): e4m3 has 4 bits, f16 11, and a row stays
 // exact down to 2^-15 of the tile's largest row, and right to 2^-13 of its own largest value down to 2^-20.  What is
 // left is one factor per tile, so a score costs one multiply-add and one exponent: P = 2^(x - m + nv - ref + 7), ref the
 // running maximum of the tiles' nv, m a lazy maximum that no x passes by more than 8 (P < 2^15).  The 7 keeps f16's
 // full precision down to 2^-21.  (Raising m costs a pass over O in tensor memory: with 2 in place of the 8 most tiles did.
-// Both powers of two applied to the scores, with two exponents each, made the softmax the bound: 254 us.)  O carries 2^-ref
+// Both powers of two applied to the scores, with two exponents each, took twice the softmax's time.)  O carries 2^-ref
 // and 2^7 until the end.
 // A row whose K or V is NaN becomes a NaN key and a zero value, which reaches the queries that see it and no others.
 #pragma once
@@ -31,14 +35,17 @@
 
 namespace reax {
 
-constexpr int PF_BN = 64, PF_ROWS = 128, PF_THREADS = 14 * 32;
+constexpr int PF_BN = 64, PF_ROWS = 128, PF_THREADS = 15 * 32;
 
 template <int D>
 struct PrefixCfg {
   static constexpr uint32_t KV_BYTES = PF_BN * D * 2;
   static constexpr uint32_t Q_COL = 128, O_COL = 256, TMEM_COLS = 512;  // S (then P) at columns 0 and 64
-  static constexpr int RAW = 2 * PF_BN * D, EXP = 2 * PF_BN;  // a tile as it lies in the cache: rows of K, of V; their exponents
-  static constexpr int NR = D == 256 ? 2 : 4;                 // tiles of it in flight
+  static constexpr int RAW = PF_BN * D, EXP = 2 * PF_BN;  // a tile's rows of K (or V) as they lie in the cache; both exponents
+  // Of those in flight, K and V in turn.  Even, so that a buffer's full barrier always has the same warps waiting: others could take
+  // the parity of the phase before theirs for it.
+  static constexpr int NR = D == 256 ? 6 : 8;
+  static_assert(NR % 2 == 0 && NR <= 8);
   static constexpr int SMEM = 1024 + 4 * KV_BYTES + NR * (RAW + EXP);
 };
 
@@ -53,6 +60,33 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 
+// One lane of the warp, always the same
+__device__ __forceinline__ uint32_t elect_lane() {
+  uint32_t x;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}\n" : "=r"(x));
+  return x;
+}
+// The whole warp comes here, the lane with `lead` issues.  With the warp together the compiler keeps descriptors and addresses in uniform
+// registers, which is where the instruction takes them from: a product of N = 64 every 33 cycles (the tensor core's rate), in a
+// branch of one lane every 50.
+__device__ __forceinline__ void mma_ts_lead(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accum, uint32_t lead) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accum), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit_lead(uint32_t bar, uint32_t lead) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(bar),
+      "r"(lead)
+      : "memory");
+}
+
 __device__ __forceinline__ uint32_t ld_shared_u16(uint32_t addr) {
   uint16_t x;
   asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(addr) : "memory");
@@ -64,8 +98,8 @@ template <int D>
 __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_constant__ PagedArgs a) {
   using C = PrefixCfg<D>;
   extern __shared__ uint8_t pf_raw[];
-  __shared__ __align__(8) uint64_t bars[24];
-  __shared__ uint32_t sgran[4];  // which of a raw tile's four groups of 16 keys were copied
+  __shared__ __align__(8) uint64_t bars[12 + 2 * C::NR];
+  __shared__ uint32_t sgran[C::NR];  // which of a raw buffer's four groups of 16 keys were copied
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   __shared__ int skn[4], svn[4];          // a tile's largest nk and nv
@@ -79,16 +113,14 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
   const int c0 = split * a.pchunk, c1 = min(a.Lp, c0 + a.pchunk), ntiles = (c1 - c0 + PF_BN - 1) / PF_BN;
   const int rows = a.B * a.M;
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
-  // kfull 0,1  vfull 2,3  kempty 4,5  vempty 6,7  s_ready 8,9  p_ready 10,11  pv_done 12,13  drain 14  q_ready 15
-  // raw_full 16..19  raw_empty 20..23
+  // kfull 0,1  vfull 2,3  s_done 4,5  pv_done 6,7  p_ready 8,9  drain 10  q_ready 11  raw_full 12..  raw_empty 12 + NR..
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 4; ++i) mbar_init(bar(i), 8);
-    for (int i = 4; i < 10; ++i) mbar_init(bar(i), 1);
-    mbar_init(bar(10), 4);
+    for (int i = 0; i < 4; ++i) mbar_init(bar(i), 4), mbar_init(bar(4 + i), 1);
+    mbar_init(bar(8), 4);
+    mbar_init(bar(9), 4);
+    mbar_init(bar(10), 1);
     mbar_init(bar(11), 4);
-    for (int i = 12; i < 15; ++i) mbar_init(bar(i), 1);
-    mbar_init(bar(15), 4);
-    for (int i = 0; i < 4; ++i) mbar_init(bar(16 + i), 1), mbar_init(bar(20 + i), 8);
+    for (int i = 0; i < C::NR; ++i) mbar_init(bar(12 + i), 1), mbar_init(bar(12 + C::NR + i), 4);
     abort_flag = 0;
     fence_mbar_init();
   }
@@ -105,21 +137,22 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
   if (warp >= 4 && warp < 12) {  // ---------------------------------------------------------------- dequantisation
     // A load of a warp covers whole rows, two (D = 256) or four, 64 bytes to four lanes.  Neighbouring groups of four lanes take
     // neighbouring rows and different 64-byte parts, so that eight lanes' loads and stores fall in different banks.
-    constexpr int RPU = 512 / D, U = 8 / RPU, NQ = D / 64;
-    const int w = warp - 4, row = w * 8 + (lane & 7), grp = lane >> 2;
+    constexpr int RPU = 512 / D, U = 16 / RPU, NQ = D / 64;
+    const bool is_v = warp >= 8;
+    const int w = warp & 3, row = w * 16 + (lane & 15), grp = lane >> 2;
     const int ur = 2 * ((grp >> 1) / NQ) + (grp & 1), quad = ((grp >> 1) + (grp & 1)) % NQ;
-    // scale: of row w * 8 + (lane & 7); all ones: a row without values, filled with `fill`
+    // scale: of row w * 16 + (lane & 15); all ones: a row without values, filled with `fill`
     auto put = [&](uint32_t buf, uint32_t raw, uint32_t scale, uint32_t fill) {
       uint4 x[U];
 #pragma unroll
-      for (int i = 0; i < U; ++i) x[i] = ld_shared_v4(raw + (w * 8 + i * RPU + ur) * D + quad * 64 + (lane & 3) * 16);
+      for (int i = 0; i < U; ++i) x[i] = ld_shared_v4(raw + (w * 16 + i * RPU + ur) * D + quad * 64 + (lane & 3) * 16);
       const bool some = __any_sync(0xffffffffu, scale == 0xffffffffu);
 #pragma unroll
       for (int i = 0; i < U; ++i) {
         const int r = i * RPU + ur;
         const uint32_t sc = __shfl_sync(0xffffffffu, scale, r);
         const uint32_t y[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-        const uint32_t dst = buf + quad * (PF_BN * 128) + (w * 8 + r) * 128;
+        const uint32_t dst = buf + quad * (PF_BN * 128) + (w * 16 + r) * 128;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           uint32_t z[4];
@@ -129,7 +162,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
             asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(z[n]) : "r"(v), "r"(sc));
           }
           if (some && sc == 0xffffffffu) z[0] = z[1] = z[2] = z[3] = fill;
-          st_shared_v4(dst + (((2 * (lane & 3) + k) ^ r) << 4), make_uint4(z[0], z[1], z[2], z[3]));
+          st_shared_v4(dst + (((2 * (lane & 3) + k) ^ (r & 7)) << 4), make_uint4(z[0], z[1], z[2], z[3]));
         }
       }
       fence_proxy_async_smem();
@@ -141,11 +174,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
       const uint32_t b = e >= -14 ? (uint32_t)(e + 15) << 10 : e >= -24 ? 1u << (e + 24) : 0u;
       return b | (b << 16);
     };
+    int rs = is_v;
+    uint32_t phase = 0;
     for (int j = 0; j < ntiles; ++j) {
-      const int s = j & 1, rs = j % C::NR;
+      const int s = j & 1;
       const uint32_t par = ((j >> 1) & 1) ^ 1;  // the buffer's previous use, done; the first two pass at once
       const uint32_t raw = sraw + rs * C::RAW, ex = sexp + rs * C::EXP;
-      if (!mbar_wait_warp(bar(16 + rs), (j / C::NR) & 1, abort, ST_TIMEOUT_ATTN)) break;
+      if (!mbar_wait_warp(bar(12 + rs), phase, abort, ST_TIMEOUT_ATTN)) break;
       // exponents of keys 2 lane, 2 lane + 1; NaN rows and keys that do not exist take no part in the maxima
       const bool even_ok = (sgran[rs] >> (lane >> 3)) & 1u && c0 + j * PF_BN + 2 * lane < c1;
       const bool odd_ok = even_ok && c0 + j * PF_BN + 2 * lane + 1 < c1;
@@ -161,98 +196,98 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
       const uint32_t kp = __shfl_sync(0xffffffffu, kb, row >> 1), vp = __shfl_sync(0xffffffffu, vb, row >> 1);
       const int nk = row & 1 ? kp >> 8 : kp & 255u, nv = row & 1 ? vp >> 8 : vp & 255u;
       const bool none = nk == 255 || nv == 255 || !(((row & 1 ? odd : even) >> (row >> 1)) & 1u);
-      if (!mbar_wait_warp(bar(4 + s), par, abort, ST_TIMEOUT_ATTN)) break;
-      put(sk + s * C::KV_BYTES, raw, none ? 0xffffffffu : scale_of(nk, kn), 0x7e007e00u);  // NaN where there is no key either: masked
+      if (!mbar_wait_warp(bar((is_v ? 6 : 4) + s), par, abort, ST_TIMEOUT_ATTN)) break;
+      const uint32_t scale = none ? 0xffffffffu : is_v ? scale_of(nv, vn) : scale_of(nk, kn);
+      // a key's NaN where there is no key either: masked
+      put((is_v ? sv : sk) + s * C::KV_BYTES, raw, scale, is_v ? 0u : 0x7e007e00u);
       // For the softmax, which reads it after S_j.  Four of them: this one's place was read by the softmax of j - 4, which was done
       // before S_{j-2} was issued, whose end K_j's buffer waited for.
-      if (w == 0 && lane == 0) {
+      if (warp == 4 && lane == 0) {
         skn[j & 3] = kn - 127;
         svn[j & 3] = vn - 127;
         seven[j & 3] = even;
         sodd[j & 3] = odd;
       }
-      if (lane == 0) mbar_arrive(bar(s));
-      if (!mbar_wait_warp(bar(6 + s), par, abort, ST_TIMEOUT_ATTN)) break;
-      put(sv + s * C::KV_BYTES, raw + PF_BN * D, none ? 0xffffffffu : scale_of(nv, vn), 0u);
       if (lane == 0) {
-        mbar_arrive(bar(2 + s));
-        mbar_arrive(bar(20 + rs));
+        mbar_arrive(bar((is_v ? 2 : 0) + s));
+        mbar_arrive(bar(12 + C::NR + rs));
       }
+      rs += 2;
+      if (rs >= C::NR) rs -= C::NR, phase ^= 1;
     }
-  } else if (warp == 13) {  // --------------------------------------------------------------------- copies
-    // lanes 0-3: K rows of a group of 16 keys, 4-7: V rows, 8-11 and 12-15: their exponents
-    const int gr = lane & 3, what = (lane >> 2) & 3;
-    const uint8_t* src = what == 0 ? a.kc + h * a.cH : what == 1 ? a.vc + h * a.cH : what == 2 ? a.ke + h * a.eH : a.ve + h * a.eH;
-    const long long pstride = what < 2 ? a.cP : a.eP;
-    const int each = what < 2 ? D : 1;  // bytes per key
+  } else if (warp >= 13) {  // --------------------------------------------------------------------- copies
+    // lanes 0-3: rows of a group of 16 keys, 4-7 and 8-11: their exponents (both, for K and for V: a NaN in one leaves out the other)
+    // rows of a copy: what of a tile surely lies in one page
+    const int piece = a.page % 64 == 0 ? 64 : a.page % 32 == 0 ? 32 : 16;
+    const int gr = lane & 3, what = lane >> 2, first = gr * 16 & ~(piece - 1);
+    const bool mine = first == gr * 16;
+    const bool is_v = warp == 14;
+    const uint8_t *rows_of = (is_v ? a.vc : a.kc) + h * a.cH, *exps = (what == 1 ? a.ke : a.ve) + h * a.eH;
     CopyLedger ledger;
     int off = 0;
     auto page_of = [&](int j) {
-      const int key = c0 + j * PF_BN + gr * 16, pi = a.shift >= 0 ? key >> a.shift : key / a.page;
+      const int key = c0 + j * PF_BN + first, pi = a.shift >= 0 ? key >> a.shift : key / a.page;
       off = key - pi * a.page;
       return key < c1 ? a.prefix[pi] : -1;
     };
-    int id = page_of(0);
+    int id = page_of(0), rs = is_v;
+    uint32_t phase = 0;
     for (int j = 0; j < ntiles; ++j) {
-      const int s = j % C::NR;
       const bool ok = id >= 0 && id < a.pages;
-      if (!ok && c0 + j * PF_BN + gr * 16 < c1) record_status(ST_BAD_PAGE);
-      const uint8_t* from = src + (ok ? id : 0) * pstride + (long long)off * each;
+      if (!ok && c0 + j * PF_BN + first < c1) record_status(ST_BAD_PAGE);
+      const uint8_t* from = what ? exps + (ok ? id * a.eP + off : 0) : rows_of + (ok ? id * a.cP + (long long)off * D : 0);
       if (j + 1 < ntiles) id = page_of(j + 1);
-      if (!mbar_wait_warp(bar(20 + s), ((j / C::NR) & 1) ^ 1, abort, ST_TIMEOUT_ATTN)) break;
       const uint32_t groups = __ballot_sync(0xffffffffu, ok) & 15u;
+      if (!mbar_wait_warp(bar(12 + C::NR + rs), phase ^ 1, abort, ST_TIMEOUT_ATTN)) break;
       if (lane == 0) {
-        sgran[s] = groups;
-        ledger.arm(s, (j / C::NR) & 1);
-        mbar_arrive_expect_tx(bar(16 + s), __popc(groups) * 2 * 16 * (D + 1));
+        sgran[rs] = groups;
+        ledger.arm(rs, phase);
+        mbar_arrive_expect_tx(bar(12 + rs), __popc(groups) * 16 * (D + 2));
       }
       __syncwarp();
-      if (ok && lane < 16)
-        bulk_load(what < 2 ? sraw + s * C::RAW + (what * PF_BN + gr * 16) * D : sexp + s * C::EXP + (what - 2) * PF_BN + gr * 16, from,
-                  16 * each, bar(16 + s));
+      if (ok && mine && what < 3)
+        bulk_load(what ? sexp + rs * C::EXP + (what - 1) * PF_BN + first : sraw + rs * C::RAW + first * D, from, what ? piece : piece * D,
+                  bar(12 + rs));
+      rs += 2;
+      if (rs >= C::NR) rs -= C::NR, phase ^= 1;
     }
-    if (lane == 0) ledger.drain([&](int i) { return bar(16 + i); });  // no copy outlives the CTA
+    if (lane == 0) ledger.drain([&](int i) { return bar(12 + i); });  // no copy outlives the CTA
     __syncwarp();
   } else if (warp == 12) {  // --------------------------------------------------------------------- MMA issue
-    if (lane == 0) {
-      constexpr uint32_t IDESC_S = idesc_f16(PF_ROWS, PF_BN), IDESC_PV = idesc_f16(PF_ROWS, D, /*b_mn_major=*/1);
-      bool live = true;
-      for (int j = 0; j <= ntiles && live; ++j) {
-        if (j < ntiles) {
-          const int s = j & 1;
-          live = (j > 0 || mbar_wait(bar(15), 0, abort, ST_TIMEOUT_ATTN)) && mbar_wait(bar(s), (j >> 1) & 1, abort, ST_TIMEOUT_ATTN);
-          if (!live) break;
-          tc_fence_after();
+    constexpr uint32_t IDESC_S = idesc_f16(PF_ROWS, PF_BN), IDESC_PV = idesc_f16(PF_ROWS, D, /*b_mn_major=*/1);
+    const uint32_t lead = elect_lane();
+    for (int j = 0; j <= ntiles; ++j) {
+      if (j < ntiles) {
+        const int s = j & 1;
+        if (j == 0 && !mbar_wait_warp(bar(11), 0, abort, ST_TIMEOUT_ATTN)) break;
+        if (!mbar_wait_warp(bar(s), (j >> 1) & 1, abort, ST_TIMEOUT_ATTN)) break;
+        tc_fence_after();
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk)
-            mma_bf16_ts(tmem + s * 64, tmem + C::Q_COL + kk * 8,
-                        sw128_desc(sk + s * C::KV_BYTES + (kk >> 2) * (PF_BN * 128) + (kk & 3) * 32), IDESC_S, kk > 0);
-          mma_commit(bar(4 + s));
-          mma_commit(bar(8 + s));
-        }
-        if (j > 0) {
-          const int i = j - 1, s = i & 1;
-          live = mbar_wait(bar(10 + s), (i >> 1) & 1, abort, ST_TIMEOUT_ATTN) &&
-                 mbar_wait(bar(2 + s), (i >> 1) & 1, abort, ST_TIMEOUT_ATTN);
-          if (!live) break;
-          tc_fence_after();
-#pragma unroll
-          for (int kk = 0; kk < PF_BN / 16; ++kk)
-            mma_bf16_ts(tmem + C::O_COL, tmem + s * 64 + kk * 8,
-                        sw128_desc(sv + s * C::KV_BYTES + kk * 2048, /*lbo=*/PF_BN * 128, /*sbo=*/1024), IDESC_PV, i > 0 || kk > 0);
-          mma_commit(bar(6 + s));
-          mma_commit(bar(12 + s));
-        }
+        for (int kk = 0; kk < D / 16; ++kk)
+          mma_ts_lead(tmem + s * 64, tmem + C::Q_COL + kk * 8,
+                      sw128_desc(sk + s * C::KV_BYTES + (kk >> 2) * (PF_BN * 128) + (kk & 3) * 32), IDESC_S, kk > 0, lead);
+        mma_commit_lead(bar(4 + s), lead);
       }
-      // whatever was issued ends before the CTA gives its memory back
-      mma_commit(bar(14));
-      const long long t0 = clock64();
-      while (!mbar_try_wait(bar(14), 0))
-        if (clock64() - t0 > REAX_DRAIN_LIMIT) {
-          record_status(ST_TIMEOUT_DRAIN);
-          break;
-        }
+      if (j > 0) {
+        const int i = j - 1, s = i & 1;
+        if (!mbar_wait_warp(bar(8 + s), (i >> 1) & 1, abort, ST_TIMEOUT_ATTN)) break;
+        if (!mbar_wait_warp(bar(2 + s), (i >> 1) & 1, abort, ST_TIMEOUT_ATTN)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < PF_BN / 16; ++kk)
+          mma_ts_lead(tmem + C::O_COL, tmem + s * 64 + kk * 8,
+                      sw128_desc(sv + s * C::KV_BYTES + kk * 2048, /*lbo=*/PF_BN * 128, /*sbo=*/1024), IDESC_PV, i > 0 || kk > 0, lead);
+        mma_commit_lead(bar(6 + s), lead);
+      }
     }
+    // whatever was issued ends before the CTA gives its memory back
+    mma_commit_lead(bar(10), lead);
+    const long long t0 = clock64();
+    while (!mbar_try_wait(bar(10), 0))
+      if (clock64() - t0 > REAX_DRAIN_LIMIT) {
+        record_status(ST_TIMEOUT_DRAIN);
+        break;
+      }
     __syncwarp();
   } else if (warp < 4) {  // ----------------------------------------------------------------------- softmax
     const int row = warp * 32 + lane, R = R0 + row;
@@ -286,13 +321,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
     tmem_wait_st();
     tc_fence_before();
     __syncwarp();
-    if (lane == 0) mbar_arrive(bar(15));
+    if (lane == 0) mbar_arrive(bar(11));
     float m = -INFINITY, l = 0.f;
     int ref = -127;
     bool live = true;
     for (int j = 0; j < ntiles; ++j) {
       const int s = j & 1;
-      live = mbar_wait_warp(bar(8 + s), (j >> 1) & 1, abort, ST_TIMEOUT_ATTN);
+      live = mbar_wait_warp(bar(4 + s), (j >> 1) & 1, abort, ST_TIMEOUT_ATTN);
       if (!live) break;
       tc_fence_after();
       uint32_t x[64];
@@ -322,7 +357,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
         m = mn;
         if (j > 0) {
           const float ao = al * ex2_approx((float)(ref - rn));
-          live = mbar_wait_warp(bar(12 + (s ^ 1)), ((j - 1) >> 1) & 1, abort, ST_TIMEOUT_ATTN);
+          live = mbar_wait_warp(bar(6 + (s ^ 1)), ((j - 1) >> 1) & 1, abort, ST_TIMEOUT_ATTN);
           if (!live) break;
           tc_fence_after();
 #pragma unroll 1
@@ -356,9 +391,9 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(10 + s));
+      if (lane == 0) mbar_arrive(bar(8 + s));
     }
-    if (live) live = mbar_wait_warp(bar(12 + ((ntiles - 1) & 1)), ((ntiles - 1) >> 1) & 1, abort, ST_TIMEOUT_ATTN);
+    if (live) live = mbar_wait_warp(bar(6 + ((ntiles - 1) & 1)), ((ntiles - 1) >> 1) & 1, abort, ST_TIMEOUT_ATTN);
     const long long out = (long long)(a.splits + split) * a.B * a.H * a.M + ((long long)b * a.H + h) * a.M + mr;
     if (live) {
       tc_fence_after();

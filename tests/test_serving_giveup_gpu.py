@@ -1,8 +1,8 @@
 """The shared-prefix kernel's pipeline gives up, unwinds and reports.
 
-libreax_decode is rebuilt here with the wait limit cut to 300 cycles and the suspension between checks to 0.5 us, less than a
-tile's copy out of memory takes, so waits of every role run out.  The roles must then unwind as built: the abort flag stops
-the others at their next wait, the copying warp waits for every copy it armed, the issuing thread for every MMA, tensor memory
+libreax_decode is rebuilt here with the wait limit cut to 300 cycles and waits that poll, so that every wait for a tile's copy,
+or for what is made of it, runs out.  The roles must then unwind as built: the abort flag stops
+the others at their next wait, the copying warp waits for every copy it armed, the issuing warp for every MMA, tensor memory
 is released and the CTAs exit.  Checked: the launch returns, the status word holds the timeout code (and reading clears it), the
 rows that were not computed are NaN, and the same context then computes correctly with the normal build.  No fault and no
 hang is involved: only bounded waits run out."""
@@ -27,7 +27,7 @@ def short_limit():
     nvcc = shutil.which("nvcc") or B.NVCC
     with tempfile.TemporaryDirectory() as td:
         so = os.path.join(td, "libreax_decode_shortwait.so")
-        cmd = ([nvcc] + B.ARCH + B.NVCC_FLAGS + ["-DREAX_WAIT_LIMIT=(300ll)", "-DREAX_WAIT_SLEEP_NS=500",
+        cmd = ([nvcc] + B.ARCH + B.NVCC_FLAGS + ["-DREAX_WAIT_LIMIT=(300ll)", "-DREAX_WAIT_POLL",
                                                   os.path.join(B.CSRC, "decode_lib.cu"), "-o", so])
         subprocess.run(cmd, check=True, capture_output=True)
         lib = ctypes.CDLL(so)
