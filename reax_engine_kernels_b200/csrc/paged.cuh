@@ -553,8 +553,8 @@ __global__ void __launch_bounds__(128, PagedCfg<D, RT>::CTAS) paged_kernel(const
 }
 
 // Joins the chunks' partial outputs: one CTA per row; D / 4 threads take four values each, 128 / (D / 4) groups of them every other
-// chunk.  ROWS: rows per CTA of the launch that made them.
-template <int D, int ROWS>
+// chunk.  AHEAD: partial outputs a thread asks for before the chunks' sums are compared.
+template <int D, int AHEAD>
 __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedArgs a) {
   constexpr int TPG = D / 4, GROUPS = 128 / TPG;
   __shared__ float red[4], sum_s[GROUPS];
@@ -562,11 +562,18 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, grp = threadIdx.x / TPG, d = threadIdx.x % TPG * 4;
   const long long rows = (long long)a.B * a.H * a.M, R = blockIdx.x;
   const int r = (int)(R % a.M), h = (int)(R / a.M % a.H), b = (int)(R / a.M / a.H);
-  const int n = paged_visible<ROWS>(a, b, r & ~(ROWS - 1), lane);
+  const int n = paged_visible<16>(a, b, r & ~15, lane);  // the tile's, of 8 rows too: there are none behind them then
   pdl_wait();
   const int chunk = paged_chunk(a, n), mine = (n + chunk - 1) / chunk, total = mine + a.psplits;
   if (a.psplits == 0 && n <= chunk) return;  // written by its only chunk
   auto slot = [&](int i) { return (i < mine ? i : a.splits + i - mine) * rows + R; };
+  // the first partial outputs, while the sums are compared
+  float4 ahead[AHEAD];
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k) {
+    const int i = grp + k * GROUPS;
+    ahead[k] = i < total ? *reinterpret_cast<const float4*>(a.part + slot(i) * D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
   float top = -INFINITY;
   bool nan = false;
   for (int i = threadIdx.x; i < total; i += 128) {
@@ -582,8 +589,15 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
   const float ref = nan ? __uint_as_float(0x7fc00000u) : finite_or_zero(top);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k) {
+    const int i = grp + k * GROUPS;
+    const float w = i < total ? ex2_approx(a.lse[slot(i)] - ref) : 0.f;
+    sum += w;
+    acc.x += w * ahead[k].x, acc.y += w * ahead[k].y, acc.z += w * ahead[k].z, acc.w += w * ahead[k].w;
+  }
 #pragma unroll 8
-  for (int i = grp; i < total; i += GROUPS) {
+  for (int i = grp + AHEAD * GROUPS; i < total; i += GROUPS) {
     const long long at = slot(i);
     const float w = ex2_approx(a.lse[at] - ref);
     const float4 x = *reinterpret_cast<const float4*>(a.part + at * D + d);

@@ -91,8 +91,13 @@ inline int paged_go(const reax::PagedArgs& a, cudaStream_t st) {
     if (int rc = prefix_tiled(a.B, a.M) ? prefix_launch<D>(a, st) : paged_launch<D, 2, true>(a, st)) return rc;
   if (int rc = a.M <= 8 ? paged_launch<D, 1, false>(a, st) : paged_launch<D, 2, false>(a, st)) return rc;
   if (a.splits + a.psplits > 1 && !a.cluster) {
-    const dim3 rows((unsigned)((long long)a.B * a.H * a.M));
-    return launch_dependent(a.M <= 8 ? reax::paged_join_kernel<D, 8> : reax::paged_join_kernel<D, 16>, rows, 128, 0, true, st, 1, a);
+    // Eight partial outputs ahead where all rows' CTAs fit the GPU at 64 registers (one sequence of 16384 keys, 32 rows: 15.9 us with
+    // none, 15.5 with two, 14.3 with eight); two, in 32 registers, where they would not (64 sequences, 2048 rows: 21.2, 21.0 and 24.0)
+    const long long rows = (long long)a.B * a.H * a.M;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    return launch_dependent(rows <= 8LL * device_sms(dev) ? reax::paged_join_kernel<D, 8> : reax::paged_join_kernel<D, 2>, dim3((unsigned)rows),
+                            128, 0, true, st, 1, a);
   }
   return 0;
 }
