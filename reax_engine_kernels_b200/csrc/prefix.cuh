@@ -17,8 +17,8 @@
 // At D = 256 a tile takes 2150 cycles, what the softmax's four warps take from S to P (750 to read it and for the maximum, 1050 for 64
 // exponents a thread and P, the rest waits); the products 530 and 510 (the tensor core's rate), the conversions 1500 each, side by side.
 // What they share is the shared-memory port, where the f16 rows are written and read once (1024 cycles) and the cache's bytes pass; so q
-// and P are operands out of tensor memory.  64 questions on a shared document of 32768 tokens: 123 us, 78 of them here.  Measured
-// slower: a branch of one lane to issue the products (137 us), tiles of 128 keys, whose f16 rows leave room for one buffer each; S
+// and P are operands out of tensor memory.  64 questions on a shared document of 32768 tokens: 119 us, 78 of them here.  Measured
+// slower (in a call of then 123): a branch of one lane to issue the products (137 us), tiles of 128 keys, whose f16 rows leave room for one buffer each; S
 // as two chains side by side, which leaves q no room in tensor memory; a half to an eighth of the exponents as polynomials on the FMA
 // pipe (128 to 123.5).
 //
