@@ -24,11 +24,12 @@ inline bool prefix_tiled(int B, int M) { return (long long)B * M > 16; }
 //    long ones spread.  Even shares take 37 us where these take 25 (32 ragged sequences up to 2048 keys).  No chunk under D keys (heads of
 //    128: 128 against 256 is 23.6 against 25.0 us for 32 sequences of up to 512 keys behind a prefix, 10.1 against 11.7 for a prefix of
 //    1024 before 4 sequences, 20.6 against 20.0 for 8 of up to 4096; heads of 256, one sequence of 4096: 11.1 against 10.9);
-//    none under 1024 where the sequences alone fill half the GPU (64 of up to 1024 keys: 26 -> 23 us); no more than 32
+//    none under 1024 where the sequences alone fill half the GPU (64 of up to 1024 keys: 26 -> 23 us), or under 256 behind a prefix,
+//    where a join runs anyway (32 of up to 512 keys, heads of 256: 50.2 -> 45.5; 64 of up to 1024, heads of 128: 46.2 -> 42.8); no more than 32
 //    chunks once they are two CTAs an SM (one sequence of 65536 keys: 42 us in 205 chunks, 32 in 32).
 inline PagedPlan paged_plan(int B, int H, int M, int D, int P, int page, int Lp, int sms) {
   auto cut = [&](long long keys, long long units, int resident, int& chunk, int& splits) {
-    const long long slots = (long long)sms * resident, floor = 2 * units > slots ? 1024 : D;
+    const long long slots = (long long)sms * resident, floor = 2 * units > slots ? (Lp ? 256 : 1024) : D;
     const long long most = 2LL * sms > 32 * units ? (2LL * sms + units - 1) / units : 32;
     const long long three = (3 * slots + units - 1) / units, want = three < most ? three : most;
     const long long c = ((keys + want - 1) / want + 63) / 64 * 64;
