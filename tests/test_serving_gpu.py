@@ -379,6 +379,31 @@ def test_page_ids_out_of_range_are_not_seen_and_reported(G, Lp):
     assert_attention(o, q, c, table, 0.1, qpos, G, prefix if Lp else None, Lp, bad=(n, -1, 1 << 30))
 
 
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("page,Lp", [(16, 1001), (48, 700), (64, 1000), (96, 1001), (128, 129), (192, 1151), (256, 1)])
+def test_prefix_in_pages_of_every_kind(page, Lp, D):
+    """A tile of 64 prefix keys comes in as many rows at a time as surely lie in one page: 16, 32 or 64.  One page of several is
+    missing; the tiles outnumber the buffers in flight."""
+    q, c, table, qpos, prefix = setup(41, 5, 2, 8, 1, D, page, [3, 70, 1, 33, 12], Lp)
+    bad = ()
+    if len(prefix) > 2:
+        prefix[1] = bad_id = c.k.shape[0] + 7
+        bad = (bad_id,)
+    o = rk.fmha_paged(q, c, table, D ** -0.5, qpos=qpos, G=8, prefix=prefix, prefix_len=Lp)
+    assert status() == (0x502 if bad else 0)
+    assert_attention(o, q, c, table, D ** -0.5, qpos, 8, prefix, Lp, bad=bad)
+
+
+def test_long_prefix_wraps_the_buffers():
+    """Few heads and a long prefix, so that a CTA's tiles go around its buffers many times; bits equal on a second run."""
+    for D in (128, 256):
+        q, c, table, qpos, prefix = setup(43, 5, 1, 8, 1, D, 64, [3, 70, 1, 33, 12], 64 * 64 * 20 - 5)
+        o, o2 = (rk.fmha_paged(q, c, table, D ** -0.5, qpos=qpos, G=8, prefix=prefix, prefix_len=64 * 64 * 20 - 5) for _ in range(2))
+        assert status() == 0 and torch.equal(o, o2)
+        rows = slice(0, 2)
+        assert_attention(o[rows], q[rows], c, table[rows], D ** -0.5, qpos[rows], 8, prefix, 64 * 64 * 20 - 5)
+
+
 def test_strided_operands():
     """q and out as [B, Tq, Hq, D] tensors of wider rows, folded by strides; qpos and table as slices."""
     B, H, G, Tq, D = 3, 2, 4, 2, 128
