@@ -27,6 +27,8 @@
 // they are raised to the maximum only when a p or P passes 2^8 (well within f16, and 2^-14 of the largest weight still is a
 // normal number), which one vote per 16 keys finds out.  With both exponents taken for each score, and both references
 // compared with it, a group of 16 keys took 373 instructions a warp at D = 128, a third of them for 4 scores a thread.
+// A key's P is (p_j * 2^nv_j) * 2^(m - m') in that order: behind a best key with a row of zeros (nv = -127) the two powers' product
+// is infinite, and p_j may be 0.  So keys with p_j under 2^-126 count as 0, and every other P that leaves the range raises m'.
 //
 // Fragments without shuffles: the k index of q . k may be permuted as long as q and k agree, so a thread takes 16 adjacent
 // bytes of a key row (four k16 steps at once).  ldmatrix.m16n16.trans.b8 leaves four consecutive keys of a value column in a register,
@@ -362,7 +364,7 @@ __global__ void __launch_bounds__(128, PagedCfg<D, RT>::CTAS) paged_kernel(const
           for (int e = 0; e < 2; ++e) {
             const float x = __fmaf_rn(s[rt][0][2 * r + e] + s[rt][1][2 * r + e], rs[rt][e] * ks[r], -m[rt][e]);
             p[rt][r][e] = ex2_approx(x);
-            pv[rt][r][e] = p[rt][r][e] * (vf[r] * rho[rt][e]);
+            pv[rt][r][e] = (p[rt][r][e] * vf[r]) * rho[rt][e];  // vf * rho may pass fp32's range, and p be 0
           }
       if (rare) {
 #pragma unroll
@@ -402,10 +404,10 @@ __global__ void __launch_bounds__(128, PagedCfg<D, RT>::CTAS) paged_kernel(const
             my = fmaxf(my, __shfl_xor_sync(0xffffffffu, my, k));
           }
           mx = fmaxf(mx, m[rt][e]);
-          my = fmaxf(my, mv[rt][e]);
+          my = fmaxf(fmaxf(my, mv[rt][e]), mx - 127.f);  // no less but by rounding; rho stays finite
           l[rt][e] *= ex2_approx(m[rt][e] - mx);
           al[e] = ex2_approx(mv[rt][e] - my);
-          rho[rt][e] = ex2_approx(mx - my);
+          rho[rt][e] = ex2_approx(fminf(mx - my, 127.f));
           m[rt][e] = mx;
           mv[rt][e] = my;
         }

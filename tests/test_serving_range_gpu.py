@@ -1,0 +1,103 @@
+"""Attention over the quantised cache where keys and values of very different powers of two meet, on the GPU against the
+formula in 64 bits.  What a key adds is bounded by its own weight here: no term of the tolerance takes the largest value alone.
+
+Tolerance of a row, with p_j the weights, n their number, v_j = row of e4m3 values * 2^nv_j:
+  * each weight is rounded to f16 (2^-11 of it), its exponent is off by the score's error (a dot product of D terms and its scaling
+    in fp32: (D + 8) * 2^-24 of the sum of its terms' magnitudes) and by 2^-24 of a difference of at most 150 in the log2 domain, twice,
+    with ex2's own 2^-22 (2^-16 in all), and the sum of n terms in fp32 by n * 2^-24 of their magnitudes;
+  * the divisor is off by the same without the f16 rounding;
+  * below f16's normal range a weight is off by 2^-25 against a largest p_j 2^nv_j of at least one, and e4m3 values reach 448:
+    n * 2^-25 * 448 * max_j p_j 2^nv_j;
+  * weights under 2^-126 of the row's largest are zero, and the products p_j 2^nv_j are held to 2^-150: n * 448 * 2^-150;
+  * the result is rounded to bf16, 2^-8 of it, 2^-134 below bf16's normal range."""
+import math
+
+import pytest
+import torch
+
+from reax_engine_kernels_b200 import kernels as rk
+from tests.test_serving_gpu import BF, DEV, gen, randn, status, value_ref
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def clear_status():
+    status()
+    yield
+    assert status() == 0, "a kernel reported something that the test did not expect"
+
+
+def assert_rows(o, q, c, table, scale, qpos, G, prefix=None, Lp=0, rows=None):
+    """Rows (b, r) of all heads (all of them by default) against the formula in 64 bits, within the tolerance above."""
+    B, H, M, D = q.shape
+    page = c.k.shape[2]
+    kc, vc = (t.view(torch.uint8) for t in (c.k, c.v))
+    pages = torch.zeros(0, dtype=torch.int64, device=DEV) if prefix is None else prefix.long()
+    for b, r in rows if rows is not None else [(b, r) for b in range(B) for r in range(M)]:
+        n = min(int(qpos[b, r // G]) + 1, Lp + table.shape[1] * page)
+        j = torch.arange(max(n, 0), device=DEV)
+        pg, off = torch.empty_like(j), torch.where(j < Lp, j, j - Lp) % page
+        pg[j < Lp] = pages[j[j < Lp] // page]
+        pg[j >= Lp] = table[b].long()[(j[j >= Lp] - Lp) // page]
+        k, v = (value_ref(t[pg, :, off], e[pg, :, off]) for t, e in ((kc, c.ke), (vc, c.ve)))  # [n, H, D]
+        nv = torch.pow(2.0, c.ve[pg, :, off].double() - 127).T  # [H, n]
+        qr = q[b, :, r].double()
+        p = torch.softmax(torch.einsum("hd,nhd->hn", qr, k) * scale, -1)
+        off_by = (D + 8) * 2.0 ** -24 * torch.einsum("hd,nhd->hn", qr.abs(), k.abs()) * abs(scale) + 2.0 ** -16 + n * 2.0 ** -24
+        want = torch.einsum("hn,nhd->hd", p, v)
+        tol = torch.einsum("hn,nhd->hd", p * (off_by + 2.0 ** -11), v.abs()) + (p * off_by).sum(-1)[:, None] * want.abs()
+        tol = tol * 1.01 + (n * 2.0 ** -25 * 448 * (p * nv).amax(-1) + n * 2.0 ** -126 * v.abs().amax((0, 2)))[:, None] + 2.0 ** -8 * want.abs()
+        tol = tol + n * 448 * 2.0 ** -150 + 2.0 ** -134
+        got = o[b, :, r].double()
+        assert torch.isfinite(got).all(), (b, r)
+        worst = (got - want).abs() - tol
+        assert worst.max() <= 0, (b, r, worst.max().item(), want.abs().max().item())
+
+
+def cached(g, lens, H, page, D, Lp):
+    """A cache with the pages of `lens` and of a prefix, unwritten; and what addresses it: table, prefix, the slots of the
+    prefix and of each sequence."""
+    PP = -(-Lp // page)
+    need = [-(-n // page) for n in lens]
+    c = rk.kv_cache(sum(need) + PP + 1, H, page, D)
+    order = torch.randperm(c.k.shape[0], generator=g, device=DEV)
+    table = torch.full((len(lens), max(need)), -1, dtype=torch.int32, device=DEV)
+    at, slots = PP, []
+    for b, n in enumerate(need):
+        table[b, :n] = order[at:at + n].to(torch.int32)
+        j = torch.arange(lens[b], device=DEV)
+        slots.append(order[at + j // page] * page + j % page)
+        at += n
+    j = torch.arange(Lp, device=DEV)
+    return c, table, order[:PP].to(torch.int32).contiguous(), order[j // page] * page + j % page, slots
+
+
+def along(g, B, H, M, D):
+    """A direction per head, and query rows that are multiples of it: with a scale of ln 2 / D a key t * direction has the score
+    t, 1.5 t or 2 t in the log2 domain."""
+    w = torch.where(randn(g, H, D) < 0, -1.0, 1.0)
+    f = torch.tensor([1.0, 1.5, 2.0, 1.0], device=DEV)[torch.arange(M, device=DEV) % 4]
+    return w, (w[:, None, :] * f[:, None]).expand(B, H, M, D).to(BF).contiguous()
+
+
+# rows of 8 and of 16 leave no padding row in a tile, which would raise the references for its neighbours
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("gap", [60, 104, 124, 130, 208])
+@pytest.mark.parametrize("M,Lp,L", [(8, 0, 13), (8, 0, 200), (8, 0, 3000), (16, 0, 200), (3, 0, 200), (4, 330, 20), (16, 330, 20)])
+def test_zero_value_row_under_the_largest_weight(M, Lp, L, gap, D):
+    """A key far above all others whose value row is zero, before values of 512 and more: what is left of the others' weights counts."""
+    g = gen(gap + D)
+    B, H, page = 4 if M == 4 else 1, 2, 16
+    c, table, prefix, pslots, slots = cached(g, [L] * B, H, page, D, Lp)
+    w, q = along(g, B, H, M, D)
+    for s in ([pslots] if Lp else []) + slots:
+        k, v = randn(g, len(s), H, D) * 0.3, randn(g, len(s), H, D) * 1000
+        for at in (0, 70):  # in the first group of 16 keys, and behind others
+            if at < len(s):
+                k[at], v[at] = w * float(gap), 0.0
+        rk.kv_write(k.to(BF), v.to(BF), c, s)
+    qpos = torch.full((B, M), Lp + L - 1, dtype=torch.int32, device=DEV)
+    scale = math.log(2) / D
+    o = rk.fmha_paged(q, c, table, scale, qpos=qpos, prefix=prefix if Lp else None, prefix_len=Lp)
+    assert_rows(o, q, c, table, scale, qpos, 1, prefix if Lp else None, Lp)
