@@ -23,12 +23,16 @@
 // pipe (128 to 123.5).
 //
 // The rows' powers of two go into the f16 values, relative to the tile's largest (nk, nv): e4m3 has 4 bits, f16 11, and a row stays
-// exact down to 2^-15 of the tile's largest row, and right to 2^-13 of its own largest value down to 2^-20.  What is
-// left is one factor per tile, so a score costs one multiply-add and one exponent: P = 2^(x - m + nv - ref + 7), ref the
-// running maximum of the tiles' nv, m a lazy maximum that no x passes by more than 8 (P < 2^15).  The 7 keeps f16's
-// full precision down to 2^-21.  (Raising m costs a pass over O in tensor memory: with 2 in place of the 8 most tiles did.
-// Both powers of two applied to the scores, with two exponents each, took twice the softmax's time.)  O carries 2^-ref
-// and 2^7 until the end.
+// exact down to 2^-15 of the tile's largest row.  What is left is one factor per tile, so a score costs one multiply-add and one
+// exponent: P = 2^(x + nv - mv + 7), with two lazy references per query: no x passes m by more than 8, no x + nv passes mv by more
+// (P < 2^15).  The 7 keeps f16's full precision down to 2^-21 of the largest.  (Raising a reference costs a pass over O in tensor memory: with
+// 2 in place of the 8 most tiles did.  Both powers of two applied to the scores, with two exponents each, took twice the
+// softmax's time.)  O carries 2^(7 - mv) until the end, the sum 2^-m.
+// What decides is a key's own weight: a large row that a query does not see, or that weighs nothing, must not cost the others bits.
+// So a tile whose rows of K lie more than 2^15 apart, or those of V more than 2^7, keeps its e4m3 values as they are, and each score
+// takes its key's two powers and two exponents, as in paged_kernel.  (2^7: mv may lie that far above the largest x_j + nv_j, and the 7 takes
+// it back: a weight below f16's range is off by 2^-25 of the largest, as there.)  Such a tile costs two of the common ones: the call above
+// takes 204 us with one small value row in every tile.  Rows of zeros count as 2^-127.
 // A row whose K or V is NaN becomes a NaN key and a zero value, which reaches the queries that see it and no others.
 #pragma once
 #include "paged.cuh"
@@ -102,8 +106,9 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
   __shared__ uint32_t sgran[C::NR];  // which of a raw buffer's four groups of 16 keys were copied
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
-  __shared__ int skn[4], svn[4];          // a tile's largest nk and nv
-  __shared__ uint32_t seven[4], sodd[4];  // its even and odd keys that exist
+  // a tile's largest nk and nv (bytes; + 256: its rows lie too far apart for that, the keys' own are in sown), its even and odd keys that exist
+  __shared__ uint4 stile[4];
+  __shared__ uint4 sown[4][PF_BN / 8];  // 16 bits a key: nk and, above it, nv
   pdl_wait();
   pdl_launch();  // the own keys' kernel needs nothing from here
   const uint32_t base = (smem_u32(pf_raw) + 1023u) & ~1023u;
@@ -168,10 +173,10 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
       fence_proxy_async_smem();
       __syncwarp();
     };
-    // f16x2 of 2^(n - top), 0 below f16's range
+    // f16x2 of 2^(n - top), which is -15 at least
     auto scale_of = [&](int n, int top) {
       const int e = n - top;
-      const uint32_t b = e >= -14 ? (uint32_t)(e + 15) << 10 : e >= -24 ? 1u << (e + 24) : 0u;
+      const uint32_t b = e >= -14 ? (uint32_t)(e + 15) << 10 : 1u << (e + 24);
       return b | (b << 16);
     };
     int rs = is_v;
@@ -186,27 +191,27 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
       const bool odd_ok = even_ok && c0 + j * PF_BN + 2 * lane + 1 < c1;
       const uint32_t kb = ld_shared_u16(ex + 2 * lane), vb = ld_shared_u16(ex + PF_BN + 2 * lane);
       const int k2[2] = {(int)(kb & 255u), (int)(kb >> 8)}, v2[2] = {(int)(vb & 255u), (int)(vb >> 8)};
-      int kn = 0, vn = 0;
+      int kn = 0, vn = 0, kl = 255, vl = 255;
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        if ((e ? odd_ok : even_ok) && k2[e] != 255 && v2[e] != 255) kn = max(kn, k2[e]), vn = max(vn, v2[e]);
+        if ((e ? odd_ok : even_ok) && k2[e] != 255 && v2[e] != 255)
+          kn = max(kn, k2[e]), vn = max(vn, v2[e]), kl = min(kl, k2[e]), vl = min(vl, v2[e]);
       kn = __reduce_max_sync(0xffffffffu, kn);
       vn = __reduce_max_sync(0xffffffffu, vn);
+      const bool wide = __any_sync(0xffffffffu, kl < kn - 15 || vl < vn - 7);
       const uint32_t even = __ballot_sync(0xffffffffu, even_ok), odd = __ballot_sync(0xffffffffu, odd_ok);
       const uint32_t kp = __shfl_sync(0xffffffffu, kb, row >> 1), vp = __shfl_sync(0xffffffffu, vb, row >> 1);
       const int nk = row & 1 ? kp >> 8 : kp & 255u, nv = row & 1 ? vp >> 8 : vp & 255u;
       const bool none = nk == 255 || nv == 255 || !(((row & 1 ? odd : even) >> (row >> 1)) & 1u);
       if (!mbar_wait_warp(bar((is_v ? 6 : 4) + s), par, abort, ST_TIMEOUT_ATTN)) break;
-      const uint32_t scale = none ? 0xffffffffu : is_v ? scale_of(nv, vn) : scale_of(nk, kn);
+      const uint32_t scale = none ? 0xffffffffu : wide ? 0x3c003c00u : is_v ? scale_of(nv, vn) : scale_of(nk, kn);
+      if (warp == 4 && wide) reinterpret_cast<uint32_t*>(sown[j & 3])[lane] = (kb & 255u) | (vb & 255u) << 8 | (kb >> 8) << 16 | (vb >> 8) << 24;
       // a key's NaN where there is no key either: masked
       put((is_v ? sv : sk) + s * C::KV_BYTES, raw, scale, is_v ? 0u : 0x7e007e00u);
       // For the softmax, which reads it after S_j.  Four of them: this one's place was read by the softmax of j - 4, which was done
       // before S_{j-2} was issued, whose end K_j's buffer waited for.
       if (warp == 4 && lane == 0) {
-        skn[j & 3] = kn - 127;
-        svn[j & 3] = vn - 127;
-        seven[j & 3] = even;
-        sodd[j & 3] = odd;
+        stile[j & 3] = make_uint4(kn, vn + (wide ? 256 : 0), even, odd);
       }
       if (lane == 0) {
         mbar_arrive(bar((is_v ? 2 : 0) + s));
@@ -292,11 +297,11 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
   } else if (warp < 4) {  // ----------------------------------------------------------------------- softmax
     const int row = warp * 32 + lane, R = R0 + row;
     const bool real = R < rows;
-    const int b = real ? R / a.M : 0, mr = real ? R % a.M : 0;
-    const int lim = real ? min(a.qpos[b * a.qpB + mr / a.G], a.Lp - 1) : a.Lp - 1;
+    int lim = a.Lp - 1;
+    if (real) lim = min(a.qpos[R / a.M * a.qpB + R % a.M / a.G], lim);
     const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
     // q: the row scaled by its power of two (and by the scale's sign), f16, into tensor memory
-    const uint16_t* qrow = a.q + b * a.qB + h * a.qH + mr * a.qM;
+    const uint16_t* qrow = a.q + (real ? R / a.M * a.qB + R % a.M * a.qM : 0) + h * a.qH;
     uint32_t top = 0;
 #pragma unroll 8
     for (int c = 0; c < D / 8; ++c) {
@@ -322,82 +327,141 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
     tc_fence_before();
     __syncwarp();
     if (lane == 0) mbar_arrive(bar(11));
-    float m = -INFINITY, l = 0.f;
-    int ref = -127;
+    float m = PAGED_NONE, mv = PAGED_NONE, l = 0.f;
     bool live = true;
+    // raises the references to a tile's maxima and rescales what there is
+    auto raise = [&](int j, float mx, float my) {
+      const float up = fmaxf(mx, m), upv = fmaxf(my, mv);
+      l *= ex2_approx(m - up);
+      m = up;
+      if (j > 0) {
+        const float ao = ex2_approx(mv - upv);
+        live = mbar_wait_warp(bar(7 - (j & 1)), ((j - 1) >> 1) & 1, abort, ST_TIMEOUT_ATTN);
+        if (!live) return;
+        tc_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(lanes + C::O_COL + c, o);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * ao);
+          tmem_st32_nowait(lanes + C::O_COL + c, o);
+        }
+        tmem_wait_st();
+      }
+      mv = upv;
+    };
+    auto factor = [&](uint32_t nk) {  // not 0: a masked score is -inf; nor infinite: a score may be 0
+      return fminf(fmaxf(rs * pow2_byte(nk), 0x1p-126f), 0x1.fffffep127f);
+    };
     for (int j = 0; j < ntiles; ++j) {
-      const int s = j & 1;
+      const int s = j & 1, k0 = c0 + j * PF_BN;
       live = mbar_wait_warp(bar(4 + s), (j >> 1) & 1, abort, ST_TIMEOUT_ATTN);
       if (!live) break;
       tc_fence_after();
-      uint32_t x[64];
-      tmem_ld64(lanes + s * 64, x);
-      const int k0 = c0 + j * PF_BN, vn = svn[j & 3];
-      const uint32_t even = seven[j & 3], odd = sodd[j & 3];
-      float c1s = rs * pow2_byte((uint32_t)(skn[j & 3] + 127));
-      if (c1s < 0x1p-126f) c1s = 0x1p-126f;  // not 0: a masked score is -inf
-      if (__any_sync(0xffffffffu, k0 + PF_BN - 1 > lim || (even & odd) != 0xffffffffu)) {
+      const uint4 tile = ld_shared_v4(smem_u32(&stile[j & 3]));
+      if (tile.y < 256u) {
+        // What needs nothing of S comes before it.  P = 2^(x - m + at + 7), at = nv - (mv - m): the values of a tile 2^60 smaller than
+        // what counts add nothing, but its weights still count in the sum
+        const float vn = (float)((int)tile.y - 127), c1s = factor(tile.x), most = fminf(m, mv - vn) + 8.f;
+        float at = fmaxf(vn - (mv - m), -60.f), c0s = at + 7.f - m;
+        uint32_t x[64];
+        tmem_ld64(lanes + s * 64, x);
+        if (__any_sync(0xffffffffu, k0 + PF_BN - 1 > lim || (tile.z & tile.w) != 0xffffffffu)) {
 #pragma unroll
-        for (int i = 0; i < 64; ++i)
-          if (k0 + i > lim || !(((i & 1 ? odd : even) >> (i >> 1)) & 1u)) x[i] = 0xff800000u;  // -inf
-      }
-      float t0 = -INFINITY, t1 = -INFINITY;
+          for (int i = 0; i < 64; ++i)
+            if (k0 + i > lim || !(((i & 1 ? tile.w : tile.z) >> (i >> 1)) & 1u)) x[i] = 0xff800000u;  // -inf
+        }
+        float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 64; i += 4) {
-        t0 = max3f(t0, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-        t1 = max3f(t1, __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
-      }
-      t0 = fmaxf(t0, t1);
-      const float mx = t0 == -INFINITY ? t0 : t0 * c1s;
-      if (__any_sync(0xffffffffu, mx > m + 8.f) || vn > ref) {  // raise the references, rescale what there is
-        const float mn = fmaxf(mx, m);
-        const int rn = max(vn, ref);
-        const float al = ex2_approx(m - finite_or_zero(mn));
-        l *= al;
-        m = mn;
-        if (j > 0) {
-          const float ao = al * ex2_approx((float)(ref - rn));
-          live = mbar_wait_warp(bar(6 + (s ^ 1)), ((j - 1) >> 1) & 1, abort, ST_TIMEOUT_ATTN);
+        for (int i = 0; i < 64; i += 4) {
+          t0 = max3f(t0, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+          t1 = max3f(t1, __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
+        }
+        const float mx = fmaxf(t0, t1) * c1s;
+        if (__any_sync(0xffffffffu, mx > most)) {
+          raise(j, mx, mx + vn);
           if (!live) break;
-          tc_fence_after();
-#pragma unroll 1
-          for (int c = 0; c < D; c += 32) {
-            uint32_t o[32];
-            tmem_ld32(lanes + C::O_COL + c, o);
+          at = fmaxf(vn - (mv - m), -60.f);
+          c0s = at + 7.f - m;
+        }
+        float sum = 0.f;
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * ao);
-            tmem_st32_nowait(lanes + C::O_COL + c, o);
+        for (int c = 0; c < 4; ++c) {
+          uint32_t y[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float p0 = ex2_approx(__fmaf_rn(__uint_as_float(x[c * 16 + 2 * i]), c1s, c0s));
+            const float p1 = ex2_approx(__fmaf_rn(__uint_as_float(x[c * 16 + 2 * i + 1]), c1s, c0s));
+            sum += p0 + p1;
+            y[i] = pack_f16(p0, p1);
           }
-          tmem_wait_st();
+          tmem_st8_nowait(lanes + s * 64 + c * 8, y);
         }
-        ref = rn;
-      }
-      // at = nv - ref: a tile of values 2^100 smaller than another's adds nothing, but its weights still count in the sum
-      const float at = (float)max(vn - ref, -100), c0s = at + 7.f - finite_or_zero(m);
-      float sum = 0.f;
+        l = __fmaf_rn(sum, ex2_approx(-at - 7.f), l);
+      } else {
+        // The keys' own powers of two, 16 keys at a time in two passes: as variants of the code above they took its registers and 4 us
+        // of 87 in calls without such a tile.  The first pass puts the scores back over S, the second P's chunk c over S's chunks up to c
+        auto value_n = [&](const uint4* own, int i) {  // nv + 127 of key i of the 16
+          const uint32_t w = reinterpret_cast<const uint32_t*>(own)[i >> 1];
+          return __uint_as_float(__byte_perm(w, 0x4b000000u, i & 1 ? 0x7653u : 0x7651u)) - 0x1p23f;
+        };
+        const int seen = lim - k0;
+        float mx = -INFINITY, my = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t x[16];
+          tmem_ld16_nowait(lanes + s * 64 + c * 16, x);
+          const uint4 own[2] = {sown[j & 3][2 * c], sown[j & 3][2 * c + 1]};
+          const uint32_t even = tile.z >> 8 * c, odd = tile.w >> 8 * c;
+          tmem_wait_ld16(x);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t y[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float p0 = ex2_approx(__fmaf_rn(__uint_as_float(x[c * 16 + 2 * i]), c1s, c0s));
-          const float p1 = ex2_approx(__fmaf_rn(__uint_as_float(x[c * 16 + 2 * i + 1]), c1s, c0s));
-          sum += p0 + p1;
-          y[i] = pack_f16(p0, p1);
+          for (int i = 0; i < 16; ++i) {
+            const uint32_t w = reinterpret_cast<const uint32_t*>(own)[i >> 1];
+            const float nk = __uint_as_float(max((i & 1 ? w << 7 : w << 23) & 0x7f800000u, 0x00400000u));
+            const float f = fminf(fmaxf(rs * nk, 0x1p-126f), 0x1.fffffep127f);
+            const bool is = (16 * c + i <= seen) & (((i & 1 ? odd : even) & (1u << (i >> 1))) != 0);
+            const float y = is ? __uint_as_float(x[i]) * f : -INFINITY;
+            mx = fmaxf(mx, y);
+            my = fmaxf(my, y + value_n(own, i));
+            x[i] = __float_as_uint(y);
+          }
+          tmem_st16_nowait(lanes + s * 64 + c * 16, x);
         }
-        tmem_st8_nowait(lanes + s * 64 + c * 8, y);
+        my -= 127.f;
+        tmem_wait_st();
+        if (__any_sync(0xffffffffu, mx > m + 8.f || my > mv + 8.f)) {
+          raise(j, mx, my);
+          if (!live) break;
+        }
+        const float cv = 7.f - 127.f - mv;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t x[16], y[8];
+          tmem_ld16_nowait(lanes + s * 64 + c * 16, x);
+          const uint4 own[2] = {sown[j & 3][2 * c], sown[j & 3][2 * c + 1]};
+          tmem_wait_ld16(x);
+          float sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            const float x0 = __uint_as_float(x[i]), x1 = __uint_as_float(x[i + 1]);
+            sum += ex2_approx(x0 - m) + ex2_approx(x1 - m);
+            y[i >> 1] = pack_f16(ex2_approx(x0 + (value_n(own, i) + cv)), ex2_approx(x1 + (value_n(own, i + 1) + cv)));
+          }
+          l += sum;
+          tmem_st8_nowait(lanes + s * 64 + c * 8, y);
+        }
       }
-      l = __fmaf_rn(sum, ex2_approx(-at - 7.f), l);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(8 + s));
     }
     if (live) live = mbar_wait_warp(bar(6 + ((ntiles - 1) & 1)), ((ntiles - 1) >> 1) & 1, abort, ST_TIMEOUT_ATTN);
-    const long long out = (long long)(a.splits + split) * a.B * a.H * a.M + ((long long)b * a.H + h) * a.M + mr;
+    const long long out = (long long)(a.splits + split) * a.B * a.H * a.M + ((long long)(R / a.M) * a.H + h) * a.M + R % a.M;
     if (live) {
       tc_fence_after();
-      const float fac = l == 0.f ? 0.f : pow2_byte((uint32_t)(ref + 127)) * 0x1p-7f / l;
+      const float fac = l == 0.f ? 0.f : ex2_approx(mv - m) * 0x1p-7f / l;
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         uint32_t o[32];

@@ -101,3 +101,46 @@ def test_zero_value_row_under_the_largest_weight(M, Lp, L, gap, D):
     scale = math.log(2) / D
     o = rk.fmha_paged(q, c, table, scale, qpos=qpos, prefix=prefix if Lp else None, prefix_len=Lp)
     assert_rows(o, q, c, table, scale, qpos, 1, prefix if Lp else None, Lp)
+
+
+# M = 16 rows of one sequence keep the prefix with the kernel for few rows, 64 take it to the one of 128-row tiles, whose tiles have
+# 64 keys; 8 and 16 rows without a prefix
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("M,H,Lp,L", [(8, 2, 0, 400), (16, 2, 0, 400), (16, 2, 400, 20), (64, 2, 400, 20), (64, 16, 2400, 20)])
+@pytest.mark.parametrize("kind", ["zero on top", "large value", "huge value", "tile of large values", "large key", "small values", "masked"])
+def test_rows_that_weigh_nothing_take_nothing_from_the_others(kind, M, H, Lp, L, D):
+    """Rows of another magnitude whose weight is next to nothing, or which some queries do not see: the result is the others', as
+    exactly as without them."""
+    g = gen(M + H + D)
+    page = 16
+    c, table, prefix, pslots, slots = cached(g, [L], H, page, D, Lp)
+    w, q = along(g, 1, H, M, D)
+    where, n = (pslots, Lp) if Lp else (slots[0], L)
+    if Lp:
+        rk.kv_write((randn(g, L, H, D) * 0.3 - w).to(BF), randn(g, L, H, D).to(BF), c, slots[0])
+    k, v = randn(g, n, H, D) * 0.3, randn(g, n, H, D)
+    qpos = torch.full((1, M), Lp + L - 1, dtype=torch.int32, device=DEV)
+    at = torch.arange(5, n, 64, device=DEV)  # one in each tile of 64 keys
+    if kind == "zero on top":
+        k[at], v[at] = w * 104.0, 0.0
+    elif kind == "large value":
+        k[at], v[at] = -60.0 * w, v[at] * 2.0 ** 30
+    elif kind == "huge value":
+        k[at], v[at] = -104.0 * w, v[at] * 2.0 ** 80
+    elif kind == "tile of large values":
+        k[64:128], v[64:128] = -60.0 * w, v[64:128] * 2.0 ** 40
+        k[256:320], v[256:320] = -104.0 * w, v[256:320] * 2.0 ** 70
+    elif kind == "large key":
+        k[at] = -w * 2.0 ** 30
+    elif kind == "small values":  # almost all the weight on rows 2^-30 of their neighbours
+        k[at], v[at] = 104.0 * w, v[at] * 2.0 ** -30
+        k[at + 1], v[at + 1] = 80.0 * w, v[at + 1] * 2.0 ** -20
+    else:  # the last rows of the keys, which half of the queries do not see
+        k[n - 20:], v[n - 20:] = k[n - 20:] * 2.0 ** 20, v[n - 20:] * 2.0 ** 100
+        qpos[:, :M // 2] = n - 21
+    rk.kv_write(k.to(BF), v.to(BF), c, where)
+    scale = math.log(2) / D
+    if kind == "masked":
+        q[:, :, M // 2:] *= 2.0 ** -24  # scores of fp32's range where the large keys are seen
+    o = rk.fmha_paged(q, c, table, scale, qpos=qpos, prefix=prefix if Lp else None, prefix_len=Lp)
+    assert_rows(o, q, c, table, scale, qpos, 1, prefix if Lp else None, Lp, rows=[(0, r) for r in range(0, M, max(1, M // 12))])
