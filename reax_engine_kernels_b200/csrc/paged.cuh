@@ -492,7 +492,7 @@ __global__ void __launch_bounds__(128, PagedCfg<D, RT>::CTAS) paged_kernel(const
     for (int w = 0; w < C::WARPS; ++w) top = fmaxf(top, sm[w][0][row]), topv = fmaxf(topv, sm[w][1][row]);
 #pragma unroll
     for (int w = 0; w < C::WARPS; ++w) sum += sm[w][2][row] * ex2_approx(sm[w][0][row] - top);
-    const float fac = sum == 0.f ? 0.f : ex2_approx(topv - top) / sum;
+    const float half = ex2_approx(0.5f * (topv - top)), fac = half / sum;  // in two steps: 2^-127 is below what ex2 gives
     const float lse = sum == 0.f ? -INFINITY : top + log2f(sum);
     const long long at = (PRE ? a.splits + split : split) * rows + ((long long)b * a.H + h) * a.M + mr;
 #pragma unroll
@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(128, PagedCfg<D, RT>::CTAS) paged_kernel(const
         v[e] = 0.f;
 #pragma unroll
         for (int w = 0; w < C::WARPS; ++w) v[e] += so[(w * ROWS + row) * C::OP + d + e];
-        v[e] = sum == 0.f ? 0.f : v[e] * fac;
+        v[e] = sum == 0.f ? 0.f : v[e] * half * fac;
       }
       if (direct && mr < a.M)
         *reinterpret_cast<uint4*>(a.o + b * a.oB + h * a.oH + mr * a.oM + d) =

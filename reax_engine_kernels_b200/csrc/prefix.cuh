@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
     const long long out = (long long)(a.splits + split) * a.B * a.H * a.M + ((long long)(R / a.M) * a.H + h) * a.M + R % a.M;
     if (live) {
       tc_fence_after();
-      const float fac = l == 0.f ? 0.f : ex2_approx(mv - m) * 0x1p-7f / l;
+      const float half = ex2_approx(0.5f * (mv - m)), fac = half * 0x1p-7f / l;  // in two steps, as in paged_kernel
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         uint32_t o[32];
@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
           for (int e = 0; e < 8; ++e) {
             float v[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = l == 0.f ? 0.f : __uint_as_float(o[4 * e + k]) * fac;
+            for (int k = 0; k < 4; ++k) v[k] = l == 0.f ? 0.f : __uint_as_float(o[4 * e + k]) * half * fac;
             p[e] = make_float4(v[0], v[1], v[2], v[3]);
           }
         }

@@ -103,6 +103,23 @@ def test_zero_value_row_under_the_largest_weight(M, Lp, L, gap, D):
     assert_rows(o, q, c, table, scale, qpos, 1, prefix if Lp else None, Lp)
 
 
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("M,Lp,L", [(8, 0, 200), (16, 0, 200), (8, 0, 3000), (16, 330, 20), (64, 330, 20)])
+def test_smallest_values(M, Lp, L, D):
+    """Values whose power of two is the least there is, 2^-127 (a row in some hundred 2^-126), and results below fp32's normal range."""
+    g = gen(M + D)
+    H, page = 2, 16
+    c, table, prefix, pslots, slots = cached(g, [L], H, page, D, Lp)
+    for s in ([pslots] if Lp else []) + slots:
+        rk.kv_write(randn(g, len(s), H, D).to(BF), (randn(g, len(s), H, D) * 6e-37).to(BF), c, s)
+    assert c.ve.min() == 0 and c.ve.max() <= 1
+    q = randn(g, 1, H, M, D).to(BF)
+    qpos = torch.full((1, M), Lp + L - 1, dtype=torch.int32, device=DEV)
+    o = rk.fmha_paged(q, c, table, 0.1, qpos=qpos, prefix=prefix if Lp else None, prefix_len=Lp)
+    assert o.count_nonzero() > o.numel() * 0.9
+    assert_rows(o, q, c, table, 0.1, qpos, 1, prefix if Lp else None, Lp)
+
+
 # M = 16 rows of one sequence keep the prefix with the kernel for few rows, 64 take it to the one of 128-row tiles, whose tiles have
 # 64 keys; 8 and 16 rows without a prefix
 @pytest.mark.parametrize("D", [128, 256])
