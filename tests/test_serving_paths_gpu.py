@@ -1,10 +1,13 @@
 """Launches of the serving entry points that only large batches reach, on the GPU against the formulas in 64 bits: the join
-of many rows, the longer chunks of a full GPU, more than 256 sequences of the delta rule, refused slots among long sequences."""
+of many rows, the longer chunks of a full GPU, more than 256 sequences of the delta rule, refused slots among long sequences; and
+the accuracy of the delta rule's state."""
+import math
+
 import pytest
 import torch
 
 from reax_engine_kernels_b200 import kernels as rk
-from tests.test_serving_gpu import BF, DEV, assert_delta, delta_inputs, gen, setup, status
+from tests.test_serving_gpu import BF, DEV, assert_delta, delta_inputs, delta_ref, gen, setup, status
 from tests.test_serving_range_gpu import assert_rows
 
 pytestmark = pytest.mark.gpu
@@ -74,3 +77,32 @@ def test_delta_state_slots_of_long_sequences():
     ref = torch.tensor([int(s) if i in runs else -1 for i, s in enumerate(slots)], dtype=torch.int32, device=DEV)
     live = torch.cat([torch.arange(cu[i], cu[i + 1], device=DEV) for i in runs])
     assert_delta(d, 0.1, o, state0, live, ref)
+
+
+def _cut(x):
+    """The 16 leading bits of a number: the sum of two bf16 terms."""
+    a = x.to(BF).double()
+    return a + (x - a).to(BF).double()
+
+
+def test_delta_state_holds_24_bits():
+    """The state of a prompt in its 2-norm.  Between two forgettings a chunk's state takes about 71 roundings to fp32 of half a step or
+    less (24 + 40 of the accumulations in h k and T r that make up u, 6 of the update's and one of the decay), each independent of
+    the others: sqrt(71) * 2^-24 of the norm.  (The bound per row that the other tests use grows with the number of tokens and would let
+    16 bits pass.)  The recurrence with h and u cut to 16 bits is far outside."""
+    limit = math.sqrt(71) * 2.0 ** -24
+    for lens in ([320, 500, 47], [1000]):
+        d = delta_inputs(43 + len(lens), lens, 2, 4, len(lens))
+        state0 = d["state"].clone()
+        rk.delta_state(*(d[n] for n in ("q", "k", "v", "g", "beta", "cu")), 0.1, d["state"])
+        ref = delta_ref({**d, "state": state0}, 0.1)[2]
+        for n in range(len(lens)):
+            assert (d["state"][n].double() - ref[n]).norm() <= limit * ref[n].norm(), n
+    h, cu = state0[0].double(), d["cu"].tolist()
+    rep = 2
+    for t in range(cu[0], cu[1]):
+        kt = d["k"][t].double().repeat_interleave(rep, 0)[..., None]
+        h = _cut(h * torch.exp2(d["g"][t].double())[:, None, None])
+        u = _cut(d["beta"][t].double()[:, None] * (d["v"][t].double() - (h @ kt)[..., 0]))
+        h = h + u[..., None] * kt.transpose(-1, -2)
+    assert (h - ref[0]).norm() > 2 * limit * ref[0].norm()
