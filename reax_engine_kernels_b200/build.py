@@ -16,6 +16,7 @@ import glob
 import os
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -76,18 +77,26 @@ def build_library(name: str, force: bool = False, verbose: bool = False) -> str:
 
 
 def binding_path() -> str:
-    return os.path.join(LIBDIR, "_serving.so")
+    """Named after the Python and the torch that it is built for: under another of either it is another file, which is not there."""
+    import torch
+
+    return os.path.join(LIBDIR, f"_serving.{sysconfig.get_config_var('SOABI')}.torch-{torch.__version__}.so")
 
 
-def build_binding(force: bool = False) -> str:
-    """The torch binding of libreax_decode (host C++ only, linked against that library, which lies beside it)."""
+def build_binding(force: bool = False) -> str | None:
+    """The torch binding of libreax_decode (host C++ only, linked against that library, which lies beside it).  Without a torch
+    for CUDA there is none, and the libraries are bound by their C ABI alone."""
+    try:
+        import torch
+    except ImportError:
+        torch = None
+    if torch is None or torch.version.cuda is None:
+        print("skipped _serving (the torch binding of libreax_decode): no torch with CUDA is importable")
+        return None
     src, out = os.path.join(CSRC, "serving_binding.cpp"), binding_path()
     deps = [src, os.path.join(ROOT, "include", "reax_abi.h")]
     if not force and os.path.exists(out) and os.path.getmtime(out) >= _newest(deps):
         return out
-    import sysconfig
-
-    import torch
     from torch.utils import cpp_extension as ext
 
     cuda = os.path.dirname(os.path.dirname(NVCC))
@@ -98,6 +107,8 @@ def build_binding(force: bool = False) -> str:
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"] + [f"-I{p}" for p in inc] + [src, "-o", tmp, f"-L{LIBDIR}",
             "-l:libreax_decode.so", f"-L{torch_lib}", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"])
     _run(cmd, "_serving")
+    for old in glob.glob(os.path.join(LIBDIR, "_serving*.so")):  # of another torch or Python, or of an earlier name
+        os.remove(old)
     os.replace(tmp, out)
     return out
 
@@ -107,7 +118,8 @@ def build_libraries(force: bool = False, verbose: bool = False, names=None):
     with cf.ThreadPoolExecutor(max_workers=len(names) or 1) as ex:
         futs = {ex.submit(build_library, n, force, verbose): n for n in names}
         built = [f.result() for f in cf.as_completed(futs)]
-    return built + [build_binding(force)] if "libreax_decode" in names else built
+    binding = build_binding(force) if "libreax_decode" in names else None
+    return built + [binding] if binding else built
 
 
 def build_oracle(force: bool = False):
