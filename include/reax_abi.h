@@ -193,7 +193,10 @@ int reax_kv_read(void* k, long long ksT, long long ksH, void* v, long long vsT, 
  * h*G + r % G).  Position j < prefix_len is row j % page of page prefix[j / page], the same for every sequence and computed once
  * for all of them; position prefix_len + j is row j % page of page table[b*tsB + j / page], j < P*page.  Row r of batch b sees
  * the positions <= qpos[b*qpBs + r / G]; a row that sees none is 0.  Keys of a page id outside 0 .. pages-1 are not seen, and
- * reported (0x502).  ws: 4 * splits * B*H*M * (D + 1) bytes of scratch for the call, splits = reax_fmha_paged_splits(...) of
+ * reported (0x502).  Scores, sums and accumulators are fp32 (scores have to stay in its range).  Each weight for the values is
+ * rounded to f16, by 2^-11 of it or 2^-25 of the row's largest (weight * power of two of the value row); weights under 2^-126 of the
+ * largest count as 0; an element of q under 2^-16 of its row's largest is rounded by 2^-25 of that.  This holds for every batch
+ * size, with a prefix and without.  ws: 4 * splits * B*H*M * (D + 1) bytes of scratch for the call, splits = reax_fmha_paged_splits(...) of
  * the same sizes on the current device; it may be NULL where that is 1.  prefix may be NULL where prefix_len is 0. */
 int reax_fmha_paged_splits(int B, int H, int M, int D, int P, int page, int prefix_len);
 int reax_fmha_paged(const void* q, long long qsB, long long qsH, long long qsM, const void* kc, const void* ke,
