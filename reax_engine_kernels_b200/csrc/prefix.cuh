@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefix_kernel(const __grid_cons
     const int row = warp * 32 + lane, R = R0 + row;
     const bool real = R < rows;
     int lim = a.Lp - 1;
-    if (real) lim = min(a.qpos[R / a.M * a.qpB + R % a.M / a.G], lim);
+    if (real) lim = max(min(a.qpos[R / a.M * a.qpB + R % a.M / a.G], lim), -1);  // a difference to it stays in 32 bits
     const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
     // q: the row scaled by its power of two (and by the scale's sign), f16, into tensor memory
     const uint16_t* qrow = a.q + (real ? R / a.M * a.qB + R % a.M * a.qM : 0) + h * a.qH;

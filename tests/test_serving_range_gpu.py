@@ -171,6 +171,24 @@ def test_rows_that_weigh_nothing_take_nothing_from_the_others(kind, M, H, Lp, L,
     assert_rows(o, q, c, table, scale, qpos, 1, prefix if Lp else None, Lp, rows=[(0, r) for r in range(0, M, max(1, M // 12))])
 
 
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("M", [8, 64])
+def test_rows_that_see_nothing_of_far_magnitudes(M, D):
+    """The least qpos there is, and others below the prefix or inside it, over tiles of the prefix with rows far apart."""
+    g = gen(M + D)
+    H, page, Lp, L, B = 2, 16, 400, 20, 2
+    c, table, prefix, pslots, slots = cached(g, [L] * B, H, page, D, Lp)
+    for s in [pslots] + slots:
+        v = randn(g, len(s), H, D) * torch.exp2(10.0 * randn(g, len(s), H, 1))
+        rk.kv_write(randn(g, len(s), H, D).to(BF), v.to(BF), c, s)
+    qpos = torch.full((B, M), Lp + L - 1, dtype=torch.int32, device=DEV)
+    qpos[0, :6] = torch.tensor([-(1 << 31), -(1 << 31) + 1, -2, -1, 0, 64], dtype=torch.int32)
+    q = randn(g, B, H, M, D).to(BF)
+    o = rk.fmha_paged(q, c, table, D ** -0.5, qpos=qpos, prefix=prefix, prefix_len=Lp)
+    assert o[0, :, :4].count_nonzero() == 0
+    assert_rows(o, q, c, table, D ** -0.5, qpos, 1, prefix, Lp, rows=[(0, r) for r in range(8)] + [(1, 0)])
+
+
 @pytest.mark.parametrize("seed", range(12))
 def test_far_magnitudes_drawn(seed):
     """Rows of all magnitudes and zero rows, with queries that see part of them, prefixes that end inside a tile, pages that are
